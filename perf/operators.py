@@ -180,11 +180,10 @@ def _scores_plain(s):
     at = ids.clamp(min=0)
     logp = torch.where(here, z.gather(1, at) - log_total, torch.zeros_like(log_total))
     out = {"logp": logp}
-    p = e / total
-    plogp = torch.where(p > 0, p * (z - log_total), torch.zeros_like(p))
-    entropy = -plogp.sum(1)
+    p = e / total if case["entropy"] or case["train"] else None
     if case["entropy"]:
-        out["entropy"] = entropy
+        plogp = torch.where(p > 0, p * (z - log_total), torch.zeros_like(p))
+        entropy = out["entropy"] = -plogp.sum(1)
     if case["top"]:
         value, best = _best(x, case["top"])
         live = value.float() > -math.inf
