@@ -102,3 +102,118 @@ def arm_block(variant_one_head, ids, vals, table, bilinear_w, query, values, alp
     w = torch.einsum("bkof,kof->bkof", p, values)
     z = torch.exp(torch.einsum("bfe,bkof->bkoe", x, w))
     return z.reshape(z.shape[0], -1, z.shape[-1])                               # 'b k o e -> b (k o) e'
+
+
+# ---- row operators on host tensors: the formulas of csrc/layer_norm.hip and csrc/score_rows.hip on ATen ops, in float32 or
+# ---- wider, rounded once to the tensors' type
+
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def layer_norm_fwd(x, weight, bias, eps):
+    """y, mean [.., 1], rstd [.., 1]"""
+    xw = _wide(x)
+    mean = xw.mean(-1, keepdim=True)
+    xc = xw - mean
+    rstd = 1.0 / torch.sqrt((xc * xc).mean(-1, keepdim=True) + eps)
+    y = xc * rstd
+    if weight is not None:
+        y = y * _wide(weight)
+    if bias is not None:
+        y = y + _wide(bias)
+    return y.to(x.dtype), mean, rstd
+
+
+def layer_norm_bwd(x, dy, weight, mean, rstd, need_dx, need_dw, need_db, p_dtype):
+    dyw, h = _wide(dy), (_wide(x) - mean) * rstd
+    g = dyw if weight is None else dyw * _wide(weight)
+    dx = (rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))).to(x.dtype) if need_dx else None
+    d = x.shape[-1]
+    dw = (dyw * h).reshape(-1, d).sum(0).to(p_dtype) if need_dw else None
+    db = dyw.reshape(-1, d).sum(0).to(p_dtype) if need_db else None
+    return dx, dw, db
+
+
+def _log_softmax_rows(x, temperature):
+    """log p of every score; -inf everywhere in a row of nothing but -inf; NaN in a row with a NaN or +inf"""
+    m = x.amax(-1, keepdim=True)
+    low = torch.full_like(m, torch.finfo(x.dtype).min)
+    z = (x - torch.where(m == -float("inf"), low, m)) / temperature
+    s = torch.exp(z).sum(-1, keepdim=True)
+    return torch.where(s == 0, torch.full_like(z, -float("inf")), z - torch.log(s))
+
+
+def _check_ids(ids, c, check):
+    if check and bool((ids >= c).any()):
+        raise IndexError("index out of range in self")
+
+
+def _at_ids(lp, ids):
+    """lp[.., ids]; 0 for an empty slot (a negative id), NaN past the row"""
+    c = lp.shape[-1]
+    v = lp.gather(-1, ids.long().clamp(0, c - 1))
+    v = torch.where(ids >= c, torch.full_like(v, float("nan")), v)
+    return torch.where(ids < 0, torch.zeros_like(v), v)
+
+
+def score_logprobs_fwd(X, ids, temperature, top_k, entropy):
+    lp = _log_softmax_rows(_wide(X), temperature)
+    logp = None if ids is None else _at_ids(lp, ids)
+    ent = None
+    if entropy:
+        p = torch.exp(lp)
+        ent = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(-1)
+    tl = ti = None
+    if top_k:
+        # a stable sort keeps the lowest id first among equals; -0 and 0 are equals
+        ti = torch.sort(_wide(X), dim=-1, descending=True, stable=True).indices[..., :top_k]
+        tl = lp.gather(-1, ti)
+        ti = torch.where(X.gather(-1, ti) > -float("inf"), ti, torch.full_like(ti, -1))
+        ti = torch.where(torch.isnan(tl), torch.full_like(ti, -1), ti)
+    return logp, ent, tl, ti
+
+
+def score_logprobs_bwd(X, ids, temperature, entropy, g_logp, g_entropy):
+    x = _wide(X)
+    lp = _log_softmax_rows(x, temperature)
+    p = torch.exp(lp)
+    dz = torch.zeros_like(p)
+    live = (lp > -float("inf")).any(-1, keepdim=True) | torch.isnan(lp).any(-1, keepdim=True)
+    if g_logp is not None:
+        ok = (ids >= 0) & (ids < x.shape[-1]) & live
+        g = torch.where(ok, g_logp.to(p.dtype), torch.zeros((), dtype=p.dtype))
+        dz = -p * g.sum(-1, keepdim=True)
+        dz = dz.scatter_add(-1, ids.long().clamp(0, x.shape[-1] - 1), g)
+    if g_entropy is not None:
+        t = torch.where(p == 0, torch.zeros_like(p), p * (lp + entropy.to(p.dtype).unsqueeze(-1)))
+        dz = dz - g_entropy.to(p.dtype).unsqueeze(-1) * t
+    return (dz / temperature).to(X.dtype)
+
+
+def _teacher(ids, teacher, temperature, dtype):
+    """(log q, q) over the listed slots; q = 0 in empty ones and in rows without a teacher"""
+    t = torch.where(ids < 0, torch.full((), -float("inf"), dtype=dtype), teacher.to(dtype))
+    lq = _log_softmax_rows(t, temperature)
+    return lq, torch.exp(lq)
+
+
+def distill_fwd(X, ids, teacher, temperature):
+    x = _wide(X)
+    lp = _at_ids(_log_softmax_rows(x, temperature), ids)
+    lq, q = _teacher(ids, teacher, temperature, x.dtype)
+    return temperature ** 2 * torch.where(q == 0, torch.zeros_like(q), q * (lq - lp)).sum(-1)
+
+
+def distill_bwd(X, ids, teacher, temperature, g_loss):
+    x = _wide(X)
+    c = x.shape[-1]
+    lp = _log_softmax_rows(x, temperature)
+    p = torch.exp(lp)
+    live = (lp > -float("inf")).any(-1, keepdim=True) | torch.isnan(lp).any(-1, keepdim=True)
+    _, q = _teacher(ids, teacher, temperature, x.dtype)
+    told = q.sum(-1, keepdim=True)
+    told = torch.where(told > 0, torch.ones_like(told), told)
+    d = (p * told).scatter_add(-1, ids.long().clamp(0, c - 1),
+                               torch.where((ids >= 0) & (ids < c) & live, -q, torch.zeros_like(q)))
+    return (d * (g_loss.to(x.dtype) * temperature).unsqueeze(-1)).to(X.dtype)

@@ -14,11 +14,13 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _PKG = os.path.dirname(_HERE)
 LIB_PATH = os.environ.get("ARMNET_HIP_LIB", os.path.join(_PKG, "lib", "libarmnet_hip.so"))  # env override: A/B builds
 CSRC = os.path.join(_PKG, "csrc")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_ID_RANGE, ERR_HIP = 0, -1, -2, -3, -4
 ID_I64, ID_I32 = 0, 1
 ONE_HEAD, MULTI_HEAD, GC_ARM = 0, 1, 2
+F32, BF16, F16 = 0, 1, 2                    # armnet_float_type: element types of the row operators
+MAX_ROW_IDS, MAX_ROW_TOP = 1024, 64         # ids / alternatives of one row of scores
 F_WRITE_CLAMPED_VALS, F_FAITHFUL_BISECT, F_FORCE_GENERIC, F_NO_LIN_FINISH, F_FP32_CONTRACTIONS = 0x1, 0x2, 0x4, 0x8, 0x10
 
 EXPORTS = (
@@ -38,9 +40,29 @@ EXPORTS = (
     "armnet_shard_route_fixed_epoch",
     "armnet_shard_route_fixed_hot", "armnet_shard_route_fixed_perm_hot", "armnet_shard_gather_perm_hot_f32",
     "armnet_linear_bf16x3_f32", "armnet_mlp_head_ex_f32", "armnet_entmax_rows_f32", "armnet_sibling_kernel_kind",
+    "armnet_layer_norm_fwd", "armnet_layer_norm_bwd_ws_bytes", "armnet_layer_norm_bwd", "armnet_score_ws_bytes",
+    "armnet_score_logprobs_fwd", "armnet_score_logprobs_bwd", "armnet_distill_fwd", "armnet_distill_bwd",
 )
 
 _lib = None
+
+
+def _declare_row_calls(lib):
+    """argument types of the row operators' calls: plain Python numbers and addresses are passed without wrapping each"""
+    i, l, f, p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+    view = [l, l, l, l, l, i, p]                        # rows, inner, outer_stride, row_stride, last dimension, type, x
+    ids = [f, l, p, i]                                  # temperature, ids of a row, ids, their type
+    for name, args, res in (
+            ("armnet_layer_norm_fwd", view + [i, p, p, f, p, p, p, p], i),
+            ("armnet_layer_norm_bwd_ws_bytes", [l, l], l),
+            ("armnet_layer_norm_bwd", view + [p, i, p, p, p, p, p, p, p, l, p], i),
+            ("armnet_score_ws_bytes", [l, l, i], l),
+            ("armnet_score_logprobs_fwd", view + ids + [i, p, p, p, p, p, p, l, p, p], i),
+            ("armnet_score_logprobs_bwd", view + ids + [p, p, p, p, p, p], i),
+            ("armnet_distill_fwd", view + ids + [i, p, p, p, p, l, p, p], i),
+            ("armnet_distill_bwd", view + ids + [i, p, p, p, p, p], i)):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, res
 
 
 class ArmnetNativeError(RuntimeError):
@@ -74,6 +96,7 @@ def load():
     lib.armnet_shard_route_fixed_ws_bytes.restype = ctypes.c_int64
     lib.armnet_last_hip_error.restype = ctypes.c_char_p
     lib.armnet_mlp_packed_bytes.restype = ctypes.c_int64
+    _declare_row_calls(lib)
     if lib.armnet_abi_version() != ABI_VERSION:
         raise ArmnetNativeError(f"ABI version mismatch: library {lib.armnet_abi_version()} != binding {ABI_VERSION}")
     _lib = lib
@@ -652,3 +675,173 @@ def shard_direct_perm(n, ids, R, nfeat, perm, id_status=None):
     with _on(ids, perm, id_status):
         check(load().armnet_shard_direct_perm(ctypes.c_int64(n), _ptr(ids), _id_type(ids), int(R),
                                               ctypes.c_int64(nfeat), _ptr(perm), _ptr(id_status), _stream()))
+
+
+# ---- row operators: rows are the last dimension, float32 / bfloat16 / float16 --------------------------------------------
+
+_ROW_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+def row_type(t, name):
+    try:
+        return _ROW_TYPES[t.dtype]
+    except KeyError:
+        raise ArmnetNativeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}") from None
+
+
+def row_view(x):
+    """(x or a dense copy, rows, inner, outer_stride, row_stride): the rows of x as the C calls take them.  Leading dimensions
+    that two strides describe need no copy (slices, transposed batches, expanded rows); neighbours in a row are adjacent."""
+    d = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // d, 0, 0, d
+    if d == 1 or x.stride(-1) == 1:
+        dims = []
+        for n, st in zip(x.shape[:-1], x.stride()[:-1]):
+            if n == 1:
+                continue
+            if dims and dims[-1][1] == st * n:
+                dims[-1] = (dims[-1][0] * n, st)
+            else:
+                dims.append((n, st))
+        rows = x.numel() // d
+        if len(dims) <= 1:
+            return x, rows, 0, 0, (dims[0][1] if dims else d)
+        if len(dims) == 2:
+            return x, rows, dims[1][0], dims[0][1], dims[1][1]
+    x = x.contiguous()
+    return x, x.numel() // d, 0, 0, d
+
+
+def _row_args(x, name):
+    """the leading arguments of a row call (address and all) and the tensor that has to stay alive through it"""
+    x, rows, inner, so, sr = row_view(x)
+    return x, (rows, inner, so, sr, x.shape[-1], row_type(x, name), x.data_ptr())
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _same_dense(t, shape, device, name, dtype=None):
+    if t is not None and (t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous()
+                          or (dtype is not None and t.dtype != dtype)):
+        raise ArmnetNativeError(f"{name}: expected a dense {list(shape)} tensor{'' if dtype is None else f' of {dtype}'} on "
+                                f"{device}, got {list(t.shape)} {t.dtype} on {t.device} (contiguous={t.is_contiguous()})")
+
+
+def _row_device(x):
+    if not x.is_cuda:
+        raise ArmnetNativeError(f"expected a tensor on the HIP device, got one on {x.device} (no CPU fallback)")
+    return torch.cuda.device(x.device)
+
+
+def layer_norm_fwd(x, weight, bias, eps, stats):
+    """armnet_layer_norm_fwd: y, and with `stats` the rows' mean and 1 / standard deviation (else None, None)"""
+    lib = load()
+    with _row_device(x):
+        x, view = _row_args(x, "x")
+        p = weight if weight is not None else bias
+        wt = F32 if p is None else row_type(p, "weight")
+        for t, name in ((weight, "weight"), (bias, "bias")):
+            _same_dense(t, (x.shape[-1],), x.device, name, None if p is None else p.dtype)
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        mean, rstd = torch.empty(2, view[0], device=x.device, dtype=torch.float32) if stats else (None, None)
+        if view[0]:
+            check(lib.armnet_layer_norm_fwd(*view, wt, _addr(weight), _addr(bias), eps, y.data_ptr(), _addr(mean), _addr(rstd),
+                                            torch.cuda.current_stream().cuda_stream))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(x, dy, weight, mean, rstd, need_dx, need_dw, need_db, p_dtype):
+    """armnet_layer_norm_bwd: (dx, dweight, dbias), None where not needed; the parameters' gradients in p_dtype"""
+    lib = load()
+    with _row_device(x):
+        x, view = _row_args(x, "x")
+        dy = dy.contiguous()
+        _same_dense(dy, x.shape, x.device, "dy", x.dtype)
+        d, dev = x.shape[-1], x.device
+        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_dx else None
+        dw = torch.empty(d, device=dev, dtype=p_dtype) if need_dw else None
+        db = torch.empty(d, device=dev, dtype=p_dtype) if need_db else None
+        ws, n = None, 0
+        if need_dw or need_db:
+            n = lib.armnet_layer_norm_bwd_ws_bytes(view[0], d)
+            ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        check(lib.armnet_layer_norm_bwd(*view, dy.data_ptr(), _ROW_TYPES[p_dtype] if p_dtype is not None else F32, _addr(weight),
+                                        _addr(mean), _addr(rstd), _addr(dx), _addr(dw), _addr(db), _addr(ws), n,
+                                        torch.cuda.current_stream().cuda_stream))
+    return dx, dw, db
+
+
+def score_logprobs_fwd(X, ids, temperature, top_k, entropy, stats, id_status=None):
+    """armnet_score_logprobs_fwd: ids [.., n_ids] dense or None -> (logp, entropy, top_logp, top_ids, stats), None where not
+    asked for"""
+    lib = load()
+    with _row_device(X):
+        X, view = _row_args(X, "X")
+        lead, dev = X.shape[:-1], X.device
+        n_ids = 0 if ids is None else ids.shape[-1]
+        if ids is not None:
+            _same_dense(ids, lead + (n_ids,), dev, "ids")
+        new = lambda *shape, dtype=torch.float32: torch.empty(*shape, device=dev, dtype=dtype)   # noqa: E731
+        logp = None if ids is None else new(lead + (n_ids,))
+        ent = new(lead) if entropy else None
+        tl, ti = (new(lead + (top_k,)), new(lead + (top_k,), dtype=torch.int64)) if top_k else (None, None)
+        st = new(view[0], 2) if stats else None
+        n = lib.armnet_score_ws_bytes(view[0], view[4], top_k)
+        ws = new(n, dtype=torch.uint8) if n > 0 else None
+        if view[0]:
+            check(lib.armnet_score_logprobs_fwd(*view, temperature, n_ids, _addr(ids), ID_I64 if ids is None else _id_type(ids),
+                                                top_k, _addr(logp), _addr(ent), _addr(tl), _addr(ti), _addr(st), _addr(ws), n,
+                                                _addr(id_status), torch.cuda.current_stream().cuda_stream))
+    return logp, ent, tl, ti, st
+
+
+def score_logprobs_bwd(X, ids, temperature, stats, entropy, g_logp, g_entropy):
+    """armnet_score_logprobs_bwd: the gradient of X (dense) from those of logp and entropy (either may be None)"""
+    lib = load()
+    with _row_device(X):
+        X, view = _row_args(X, "X")
+        dx = torch.empty(X.shape, device=X.device, dtype=X.dtype)
+        n_ids = 0 if ids is None else ids.shape[-1]
+        _same_dense(g_logp, () if ids is None else ids.shape, X.device, "the gradient of logp", torch.float32)
+        _same_dense(g_entropy, X.shape[:-1], X.device, "the gradient of entropy", torch.float32)
+        if view[0]:
+            check(lib.armnet_score_logprobs_bwd(*view, temperature, n_ids, _addr(ids), ID_I64 if ids is None else _id_type(ids),
+                                                stats.data_ptr(), _addr(entropy), _addr(g_logp), _addr(g_entropy), dx.data_ptr(),
+                                                torch.cuda.current_stream().cuda_stream))
+    return dx
+
+
+def distill_fwd(X, ids, teacher, temperature, stats, id_status=None):
+    """armnet_distill_fwd: (loss per row, stats for the backward or None); ids and teacher [.., k] dense"""
+    lib = load()
+    with _row_device(X):
+        X, view = _row_args(X, "X")
+        lead, dev, k = X.shape[:-1], X.device, ids.shape[-1]
+        _same_dense(ids, lead + (k,), dev, "top_ids")
+        _same_dense(teacher, lead + (k,), dev, "top_scores")
+        loss = torch.empty(lead, device=dev, dtype=torch.float32)
+        st = torch.empty(view[0], 4, device=dev, dtype=torch.float32) if stats else None
+        n = lib.armnet_score_ws_bytes(view[0], view[4], 0)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
+        if view[0]:
+            check(lib.armnet_distill_fwd(*view, temperature, k, ids.data_ptr(), _id_type(ids), row_type(teacher, "top_scores"),
+                                         teacher.data_ptr(), loss.data_ptr(), _addr(st), _addr(ws), n, _addr(id_status),
+                                         torch.cuda.current_stream().cuda_stream))
+    return loss, st
+
+
+def distill_bwd(X, ids, teacher, temperature, stats, g_loss):
+    """armnet_distill_bwd: the gradient of X (dense) from that of the rows' losses"""
+    lib = load()
+    with _row_device(X):
+        X, view = _row_args(X, "X")
+        _same_dense(g_loss, X.shape[:-1], X.device, "the gradient of the loss", torch.float32)
+        dx = torch.empty(X.shape, device=X.device, dtype=X.dtype)
+        if view[0]:
+            check(lib.armnet_distill_bwd(*view, temperature, ids.shape[-1], ids.data_ptr(), _id_type(ids),
+                                         row_type(teacher, "top_scores"), teacher.data_ptr(), stats.data_ptr(),
+                                         g_loss.data_ptr(), dx.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return dx

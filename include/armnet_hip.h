@@ -36,7 +36,9 @@ extern "C" {
  *               armnet_gather_map_stats_f32, armnet_bn_bwd_scatter_f32
  *   5  round 5: hot-row replication of the row-sharded lookup (armnet_shard_route_fixed_hot, _perm_hot,
  *               armnet_shard_gather_perm_hot_f32); armnet_linear_bf16x3_f32 (the training head's GEMMs) */
-#define ARMNET_ABI_VERSION 7
+/*   8  row operators: armnet_layer_norm_fwd / _bwd, armnet_score_logprobs_fwd / _bwd, armnet_distill_fwd / _bwd and their
+ *      workspace sizes */
+#define ARMNET_ABI_VERSION 8
 
 typedef enum armnet_status {
     ARMNET_OK = 0,
@@ -48,6 +50,9 @@ typedef enum armnet_status {
 
 /* ids may be int64 (torch.LongTensor, data_loader.py:20) or int32 */
 typedef enum armnet_id_type { ARMNET_ID_I64 = 0, ARMNET_ID_I32 = 1 } armnet_id_type;
+
+/* element type of the row operators' tensors (armnet_layer_norm_*, armnet_score_logprobs_*, armnet_distill_*) */
+typedef enum armnet_float_type { ARMNET_F32 = 0, ARMNET_BF16 = 1, ARMNET_F16 = 2 } armnet_float_type;
 
 /* model variant for parameter folding */
 typedef enum armnet_variant {
@@ -514,6 +519,73 @@ int armnet_mlp_head_f32(int64_t B, int K0, int nhid, int n_hidden, int has_final
 #define ARMNET_MLP_F_BF16X3 0x1u
 int armnet_mlp_head_ex_f32(int64_t B, int K0, int nhid, int n_hidden, int has_final, const float* x, int64_t ldx,
                            const void* packed, float* out, int64_t ldo, uint32_t flags, void* stream);
+
+/*
+ * Row operators: layer norm, log probabilities of score rows, distillation (csrc/layer_norm.hip, csrc/score_rows.hip).
+ * The reference has none of them; they stand beside its BatchNorm1d and its sparse map over a row of scores.
+ *
+ * A row is the last dimension of x, its elements adjacent.  Row r starts (r / inner) * outer_stride + (r % inner) * row_stride
+ * elements behind x (inner = 0: r * row_stride), so a view of a wider tensor needs no copy.  Everything else is dense.
+ * x is float32, bfloat16 or float16 (armnet_float_type); sums, statistics and scalar results are fp32; a value of a 16-bit type
+ * is rounded once, to nearest.  Buffers need only their elements' natural alignment.  rows, d, c < 2^31.
+ */
+
+/*
+ * y = (x - mean) * rstd * weight + bias over rows of d values; weight / bias [d] of w_type, either may be NULL; y [rows, d].
+ * mean / rstd [rows]: both (for the backward) or neither.
+ */
+int armnet_layer_norm_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t d, int x_type,
+                          const void* x, int w_type, const void* weight, const void* bias, float eps, void* y, float* mean,
+                          float* rstd, void* stream);
+/*
+ * dx [rows, d] of x's type, dweight / dbias [d] of w_type (overwritten); each may be NULL.  dy [rows, d] of x's type.  The
+ * parameter gradients need a workspace of armnet_layer_norm_bwd_ws_bytes bytes, 16-byte aligned, its content unused before and
+ * after; they are summed in a fixed order.
+ */
+int64_t armnet_layer_norm_bwd_ws_bytes(int64_t rows, int64_t d);
+int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t d, int x_type,
+                          const void* x, const void* dy, int w_type, const void* weight, const float* mean, const float* rstd,
+                          void* dx, void* dweight, void* dbias, void* workspace, int64_t ws_bytes, void* stream);
+
+/*
+ * p = softmax(x / temperature) over rows of c scores.
+ *   logp [rows, n_ids]   log p of ids [rows, n_ids] (id_type); a negative id is an empty slot: 0.  n_ids <= 1024
+ *   entropy [rows]       -sum p log p, or NULL
+ *   top_logp, top_ids    [rows, top], the `top` <= min(64, c) largest scores: log p and id, best first, ties to the lowest id
+ *   stats [rows, 2]      for the backward, or NULL
+ * A score of -inf is masked: it is never an alternative (slots past the last unmasked score hold -inf and -1).  A row of
+ * nothing but -inf has log p = -inf and entropy 0; a row with a NaN or +inf has NaN everywhere and no alternatives (-1).
+ * An id >= c has log p NaN and sets id_status like everywhere else.  1e-6 <= temperature <= 1e6.
+ * workspace: armnet_score_ws_bytes(rows, c, top) bytes, 16-byte aligned, its content unused before and after.
+ */
+int64_t armnet_score_ws_bytes(int64_t rows, int64_t c, int top);
+int armnet_score_logprobs_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
+                              const void* x, float temperature, int64_t n_ids, const void* ids, int id_type, int top,
+                              float* logp, float* entropy, float* top_logp, int64_t* top_ids, float* stats, void* workspace,
+                              int64_t ws_bytes, int32_t* id_status, void* stream);
+/* dx [rows, c] of x's type from g_logp [rows, n_ids] and g_entropy [rows] (either may be NULL; with g_entropy the forward's
+ * entropy); the same id in several slots adds up; a row of nothing but -inf has gradient 0 */
+int armnet_score_logprobs_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
+                              const void* x, float temperature, int64_t n_ids, const void* ids, int id_type,
+                              const float* stats, const float* entropy, const float* g_logp, const float* g_entropy, void* dx,
+                              void* stream);
+
+/*
+ * Distillation from a teacher's listed scores: q = softmax(teacher / temperature) over the k <= 1024 listed ids of a row (a
+ * negative id is an empty slot), p = softmax(x / temperature) over the whole row,
+ *   loss [rows] = temperature^2 * sum_k q_k (log q_k - log p[ids_k])
+ * teacher [rows, k] of t_type; stats [rows, 4] for the backward, or NULL; workspace as above with top = 0.  A row without a
+ * teacher has loss 0 and gradient 0; an id twice in a row's list counts twice.  A row of x with nothing but -inf has loss +inf
+ * (where the teacher has weight) and gradient 0.
+ */
+int armnet_distill_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
+                       const void* x, float temperature, int64_t k, const void* ids, int id_type, int t_type,
+                       const void* teacher, float* loss, float* stats, void* workspace, int64_t ws_bytes, int32_t* id_status,
+                       void* stream);
+/* dx [rows, c] of x's type from g_loss [rows] */
+int armnet_distill_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
+                       const void* x, float temperature, int64_t k, const void* ids, int id_type, int t_type,
+                       const void* teacher, const float* stats, const float* g_loss, void* dx, void* stream);
 
 #ifdef __cplusplus
 }
