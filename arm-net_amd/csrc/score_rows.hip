@@ -49,6 +49,11 @@ struct ScoreArgs {
     const float* g_entropy;    // [rows] or null
     void* dx;                  // [rows, c]
     int32_t* id_status;
+    // a row in several slices
+    int splits;
+    int64_t per;               // scores of a slice
+    float4* part;              // [rows, splits]: m, S, W
+    uint64_t* keys;            // [rows, splits, top], best first; 0: none
 };
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int id_type, int64_t i) {
@@ -61,135 +66,485 @@ __device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
     return (float)((const f16_t*)p)[i];
 }
 
-// unsigned keys in the order of (value, lowest id first); -0 and 0 are the same value.  0 is below every key.
-__device__ __forceinline__ uint64_t score_key(float v, uint32_t id) {
+// unsigned keys in the order of the values; -0 and 0 are the same value.  0 is below every key.
+__device__ __forceinline__ uint32_t value_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
-    const uint32_t k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return ((uint64_t)k << 32) | (uint32_t)~id;
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+// ... of (value, lowest id first)
+__device__ __forceinline__ uint64_t score_key(float v, uint32_t id) { return ((uint64_t)value_key(v) << 32) | (uint32_t)~id; }
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }   // results below 2^-126 are 0
+
+struct Sums {
+    float m, S, W;             // largest score, sum of e^z, sum of e^z z2
+};
+
+// moves sums to another reference m' >= m
+template <bool ENT>
+__device__ __forceinline__ void rebase(Sums& s, float m, float c2) {
+    const float d = fmaxf((s.m - m) * c2, Z_FLOOR);
+    const float f = exp2_raw(d);
+    if constexpr (ENT) s.W = f * fmaf(d, s.S, s.W);
+    s.S *= f;
+    s.m = m;
 }
 
-template <int NW>
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* scratch) {
+template <bool ENT, int N>
+__device__ __forceinline__ void add_scores(Sums& s, const float (&v)[N], float c2) {
+    float mx = v[0];
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        const uint64_t o = __shfl_xor(v, d);
-        v = o > v ? o : v;
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
+    rebase<ENT>(s, fmaxf(s.m, mx), c2);
+    float e0 = 0.f, w0 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float z = (v[i] - s.m) * c2;
+        const float e = exp2_raw(z);
+        e0 += e;
+        if constexpr (ENT) w0 = fmaf(e, fmaxf(z, Z_FLOOR), w0);
     }
-    __syncthreads();
-    if ((threadIdx.x & (WAVE - 1)) == 0) scratch[threadIdx.x / WAVE] = v;
-    __syncthreads();
-    uint64_t s = scratch[0];
+    s.S += e0;
+    if constexpr (ENT) s.W += w0;
+}
+
+// all threads' sums of a group, in every thread; scratch: 3 * NW floats of the group's own
+template <int NW, bool ENT>
+__device__ __forceinline__ Sums group_sums(Sums s, float c2, float* scratch) {
+    rebase<ENT>(s, wave_max(s.m), c2);
+    s.S = wave_sum(s.S);
+    if constexpr (ENT) s.W = wave_sum(s.W);
+    if constexpr (NW > 1) {
+        const int w = threadIdx.x / WAVE;
+        if ((threadIdx.x & (WAVE - 1)) == 0) {
+            scratch[w] = s.m;
+            scratch[NW + w] = s.S;
+            scratch[2 * NW + w] = s.W;
+        }
+        __syncthreads();
+        float m = scratch[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) s = scratch[w] > s ? scratch[w] : s;
+        for (int i = 1; i < NW; ++i) m = fmaxf(m, scratch[i]);
+        Sums t{m, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            Sums p{scratch[i], scratch[NW + i], scratch[2 * NW + i]};
+            rebase<ENT>(p, m, c2);
+            t.S += p.S;
+            t.W += p.W;
+        }
+        return t;
+    }
     return s;
 }
 
-// (m, S, sum e z2) of a row, the same in every thread
-template <typename T>
-__device__ __forceinline__ void row_sums(const ScoreArgs& a, const T* x, float* scratch, float& m, float& S, float& W) {
-    float mx = -FLT_MAX;
-    for (int i = threadIdx.x; i < a.c; i += SC_TPB) mx = fmaxf(mx, to_f32(x[i]));
-    m = block_max<SC_NW>(mx, scratch);
-    float s = 0.f, w = 0.f;
-    for (int i = threadIdx.x; i < a.c; i += SC_TPB) {
-        const float z = (to_f32(x[i]) - m) * a.c2;
-        const float e = exp2f(z);
-        s += e;
-        w = fmaf(e, fmaxf(z, Z_FLOOR), w);
+constexpr int SC_UNROLL = 4;             // pieces of 16 bytes in flight a thread
+constexpr int SC_BUF = 512;              // candidates for the alternatives
+
+template <int NW>
+struct TopScratch {
+    uint64_t key[SC_BUF];
+    int n, threads, first;
+    uint32_t cut;
+    int count[NW];
+    uint8_t who[NW * WAVE];
+};
+
+// how many threads of the group say yes, in every thread
+template <int NW>
+__device__ __forceinline__ int group_count(bool yes, int* count) {
+    int n = __popcll(__ballot(yes));
+    if constexpr (NW > 1) {
+        __syncthreads();
+        if ((threadIdx.x & (WAVE - 1)) == 0) count[threadIdx.x / WAVE] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) n += count[i];
     }
-    S = block_sum<SC_NW>(s, scratch);
-    W = block_sum<SC_NW>(w, scratch);
+    return n;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SC_TPB) score_fwd_kernel(ScoreArgs a) {
-    __shared__ float scratch[SC_NW];
-    __shared__ uint64_t scratch64[SC_NW];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* x = row_ptr<T>(a.x, r);
-        float m, S, W;
-        row_sums(a, x, scratch, m, S, W);
-        const bool some = !(S == 0.f);
-        const float l2 = some ? log2f(S) : INFINITY;
-        if (threadIdx.x == 0) {
-            if (a.entropy) a.entropy[r] = some ? LN2 * (l2 - W / S) : 0.f;
+template <int NW>
+__device__ __forceinline__ void push(TopScratch<NW>& ts, float v, uint32_t id) {
+    const int at = atomicAdd(&ts.n, 1);
+    if (at < SC_BUF) ts.key[at] = score_key(v, id);
+}
+
+// how many of a slice's scores are at least `cut`
+template <typename T, int NW>
+__device__ int count_from(const T* x, int n, float cut, int tid, TopScratch<NW>& ts) {
+    int mine = 0;
+    for (int i = tid; i < n; i += NW * WAVE) mine += to_f32(x[i]) >= cut ? 1 : 0;
+    if (tid == 0) ts.first = 0;
+    group_sync<NW>();
+    atomicAdd(&ts.first, mine);
+    group_sync<NW>();
+    const int all = ts.first;
+    group_sync<NW>();
+    return all;
+}
+
+// The `top` best scores of a slice of n scores that begins at id `id0`, as keys in ts.key[0 .. result), unordered; the result is at
+// most SC_BUF and covers the best ones.  m: the largest score that this thread met; it owns the pieces tid, tid + NT, ...
+//
+// The top-th largest of the threads' maxima is a bound: at least `top` scores reach it, and few more do (for scores in no
+// particular order top + top^2 / 2 NT).  Only the pieces of the threads whose maximum reaches it are read again, a thread's
+// pieces by the 64 lanes of a wave.  Where more than SC_BUF scores reach the bound (ties, or scores that grow along the pieces
+// of one thread), the bound is raised by halving until it fits; if ties remain, the ones with the lowest ids are taken.
+template <typename T, int NW>
+__device__ int best_scores(const T* x, int n, uint32_t id0, float m, int top, int tid, TopScratch<NW>& ts) {
+    constexpr int NT = NW * WAVE, V = Piece<T>::N;
+    const int lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int nvec = n / V, rem = n - nvec * V;
+    float* maxima = (float*)ts.key;
+    if constexpr (NW > 1) maxima[tid] = m;
+    if (tid == 0) ts.n = ts.threads = 0;
+    group_sync<NW>();
+    if (wave == 0) {                     // between lo (reached by >= top threads) and hi (by fewer), until lo is close
+        uint32_t k[NW];
+        float mn = m, mx = m;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float v = NW > 1 ? maxima[i * WAVE + lane] : m;
+            k[i] = value_key(v);
+            mn = fminf(mn, v);
+            mx = fmaxf(mx, v);
+        }
+        uint32_t lo = value_key(-wave_max(-mn)), hi = value_key(wave_max(mx)) + 1;
+        int reach = NT;
+        while (hi - lo > 1 && reach > top + 8) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) c += __popcll(__ballot(k[i] >= mid));
+            if (c >= top) { lo = mid; reach = c; } else hi = mid;
+        }
+        if (lane == 0) ts.cut = lo;
+    }
+    group_sync<NW>();
+    const uint32_t cut = ts.cut;
+    const float cutv = key_value(cut);
+    if (m >= cutv) {
+        const int at = atomicAdd(&ts.threads, 1);
+        ts.who[at] = (uint8_t)tid;
+    }
+    group_sync<NW>();
+    const int threads = ts.threads;
+    for (int i = wave; i < threads; i += NW) {
+        const int t = ts.who[i];
+        for (int64_t j = lane; j * NT + t < nvec; j += WAVE) {
+            const int at = (int)(j * NT + t);
+            float f[V];
+            Piece<T>::unpack(Piece<T>::load(x + (int64_t)at * V), f);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (f[e] >= cutv) push(ts, f[e], id0 + at * V + e);
+        }
+        if (lane == 0 && t < rem) {
+            const float v = to_f32(x[nvec * V + t]);
+            if (v >= cutv) push(ts, v, id0 + nvec * V + t);
+        }
+    }
+    group_sync<NW>();
+    int got = ts.n;
+    group_sync<NW>();
+    if (got <= SC_BUF) return got;
+
+    // too many: lo is reached by more than SC_BUF scores, hi by fewer than `top`
+    uint32_t lo = cut, hi = 0xff800001u, mid = cut + 1;            // hi: above +inf
+    bool fits = false;
+    while (hi - lo > 1) {
+        const int c = count_from<T, NW>(x, n, key_value(mid), tid, ts);
+        if (c >= top) {
+            lo = mid;
+            if (c <= SC_BUF) { fits = true; break; }
+        } else {
+            hi = mid;
+        }
+        mid = lo + (hi - lo) / 2;
+    }
+    if (tid == 0) ts.n = 0;
+    group_sync<NW>();
+    const float from = key_value(fits ? lo : hi);
+    for (int i = tid; i < n; i += NT) {
+        const float v = to_f32(x[i]);
+        if (v >= from) push(ts, v, id0 + i);
+    }
+    group_sync<NW>();
+    got = ts.n;
+    group_sync<NW>();
+    if (!fits) {                                                   // ties at lo: the lowest ids, in order
+        const float tie = key_value(lo);
+        int need = top - got;
+        for (int i0 = 0; i0 < n && need > 0; i0 += NT) {
+            const int i = i0 + tid;
+            const bool is = i < n && to_f32(x[i]) == tie;
+            const uint64_t b = __ballot(is);
+            int before = __popcll(b & ((1ull << lane) - 1)), all = __popcll(b);
+            if constexpr (NW > 1) {
+                if (lane == 0) ts.count[wave] = all;
+                __syncthreads();
+                all = 0;
+                for (int w = 0; w < NW; ++w) {
+                    if (w < wave) before += ts.count[w];
+                    all += ts.count[w];
+                }
+                __syncthreads();
+            }
+            if (is && before < need) ts.key[got + before] = score_key(tie, id0 + i);
+            const int took = all < need ? all : need;
+            got += took;
+            need -= took;
+        }
+        group_sync<NW>();
+    }
+    return got;
+}
+
+// what a row says, from its sums: log p of the ids, the entropy; or the distillation loss
+template <typename T, int NT, bool DISTILL>
+__device__ __forceinline__ void row_answer(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, int tid) {
+    const bool some = !(s.S == 0.f);
+    const float l2 = some ? log2f(s.S) : INFINITY;
+    if constexpr (!DISTILL) {
+        if (tid == 0) {
+            if (a.entropy) a.entropy[r] = some ? LN2 * (l2 - s.W / s.S) : 0.f;
             if (a.stats) {
-                a.stats[2 * r] = m;
+                a.stats[2 * r] = s.m;
                 a.stats[2 * r + 1] = l2;
             }
         }
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
+        for (int k = tid; k < a.n_ids; k += NT) {
             const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
             float v = 0.f;
             if (id >= a.c) {
                 v = NAN;
                 if (a.id_status) flag_bad_id(a.id_status);
             } else if (id >= 0) {
-                v = some ? (to_f32(x[id]) - m) * a.rt - LN2 * l2 : -INFINITY;
+                v = some ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : -INFINITY;
             }
             a.logp[r * a.n_ids + k] = v;
         }
-        uint64_t last = ~(uint64_t)0;
-        for (int k = 0; k < a.top; ++k) {              // the largest key below the last one
-            uint64_t best = 0;
-            for (int i = threadIdx.x; i < a.c; i += SC_TPB) {
-                const float v = to_f32(x[i]);
-                const uint64_t key = v > -INFINITY ? score_key(v, (uint32_t)i) : 0;
-                if (key < last && key > best) best = key;
-            }
-            last = block_max_u64<SC_NW>(best, scratch64);
-            if (threadIdx.x == 0) {
-                const int64_t id = last ? (int64_t)(uint32_t)~(uint32_t)last : -1;
-                const bool nan = S != S;
-                a.top_ids[r * a.top + k] = nan ? -1 : id;
-                a.top_logp[r * a.top + k] = nan ? NAN : id < 0 ? -INFINITY : (to_f32(x[id]) - m) * a.rt - LN2 * l2;
-            }
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(SC_TPB) distill_fwd_kernel(ScoreArgs a) {
-    __shared__ float scratch[SC_NW];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* x = row_ptr<T>(a.x, r);
-        float m, S, W;
-        row_sums(a, x, scratch, m, S, W);
-        const float l2 = S == 0.f ? INFINITY : log2f(S);
+    } else if (tid < WAVE) {                          // the list is short: one wave reads it three times
         float mt = -FLT_MAX;
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
+        for (int k = tid; k < a.n_ids; k += WAVE) {
             const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
             if (id >= 0) mt = fmaxf(mt, load_any(a.teacher, a.t_type, r * a.n_ids + k));
             if (id >= a.c && a.id_status) flag_bad_id(a.id_status);
         }
-        mt = block_max<SC_NW>(mt, scratch);
+        mt = wave_max(mt);
         float st = 0.f;
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
+        for (int k = tid; k < a.n_ids; k += WAVE) {
             const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
-            if (id >= 0) st += exp2f((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2);
+            if (id >= 0) st += exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2);
         }
-        st = block_sum<SC_NW>(st, scratch);
+        st = wave_sum(st);
         const float lt = st == 0.f ? INFINITY : log2f(st);
         float loss = 0.f;
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
+        for (int k = tid; k < a.n_ids; k += WAVE) {
             const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
             if (id < 0) continue;
             const float zt = load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt;
-            const float q = exp2f(zt * a.c2 - lt);
-            const float lp = id < a.c ? (to_f32(x[id]) - m) * a.rt - LN2 * l2 : NAN;
+            const float q = exp2_raw(zt * a.c2 - lt);
+            const float lp = id < a.c ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : NAN;
             if (!(q == 0.f)) loss = fmaf(q, (zt * a.rt - LN2 * lt) - lp, loss);
         }
-        loss = block_sum<SC_NW>(loss, scratch) * (a.t * a.t);
-        if (threadIdx.x == 0) {
+        loss = wave_sum(loss) * (a.t * a.t);
+        if (tid == 0) {
             a.loss[r] = loss;
             if (a.stats) {
-                a.stats[4 * r + 0] = m;
+                a.stats[4 * r + 0] = s.m;
                 a.stats[4 * r + 1] = l2;
                 a.stats[4 * r + 2] = mt;
                 a.stats[4 * r + 3] = lt;
             }
         }
     }
+}
+
+// orders `got` unordered keys and writes the best `top`: as a row's alternatives, or (keys != null) as keys
+template <typename T, int NT>
+__device__ __forceinline__ void write_best(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, const uint64_t* buf, int got,
+                                           uint64_t* keys, int tid) {
+    const float ll = LN2 * log2f(s.S);
+    const bool nan = s.S != s.S;
+    for (int i = tid; i < got; i += NT) {
+        const uint64_t mine = buf[i];
+        int rank = 0;
+        for (int j = 0; j < got; ++j) rank += buf[j] > mine ? 1 : 0;
+        if (rank >= a.top) continue;
+        if (keys) {
+            keys[rank] = mine;
+        } else {
+            const uint32_t id = ~(uint32_t)mine;
+            a.top_ids[r * a.top + rank] = nan ? -1 : (int64_t)id;
+            a.top_logp[r * a.top + rank] = nan ? NAN : (to_f32(x[id]) - s.m) * a.rt - ll;
+        }
+    }
+    for (int i = got + tid; i < a.top; i += NT) {
+        if (keys) {
+            keys[i] = 0;
+        } else {
+            a.top_ids[r * a.top + i] = -1;
+            a.top_logp[r * a.top + i] = nan ? NAN : -INFINITY;
+        }
+    }
+}
+
+// NW waves a slice of a row; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best keys
+template <typename T, int NW, bool ENT, bool TOP, bool DISTILL>
+__global__ void __launch_bounds__(SC_TPB) score_fwd_kernel(ScoreArgs a) {
+    constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
+    __shared__ float scratch[GROUPS][3 * NW];
+    __shared__ TopScratch<NW> top_scratch[TOP ? GROUPS : 1];
+    const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1);
+    const int64_t units = a.rows * a.splits;
+    for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
+        const int64_t r = a.splits == 1 ? unit : unit / a.splits;
+        const int64_t from = (unit - r * a.splits) * a.per;
+        const T* row = row_ptr<T>(a.x, r);
+        const T* x = row + from;
+        const int n = (int)(from + a.per < a.c ? a.per : a.c - from);
+        const int nvec = n / V, rem = n - nvec * V;
+        Sums s{-FLT_MAX, 0.f, 0.f};
+        int64_t j = tid;
+        const T* p = x + (int64_t)tid * V;
+        for (; j - tid + U * NT <= nvec; j += U * NT, p += (int64_t)U * NT * V) {
+            u32x4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = Piece<T>::load(p + (int64_t)u * NT * V);
+            float v[U * V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) Piece<T>::unpack(raw[u], *(float(*)[V])(v + u * V));
+            add_scores<ENT>(s, v, a.c2);
+        }
+        if (j - tid < nvec) {                         // the last pieces: past the end the last one again, masked
+            u32x4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = j + u * NT;
+                raw[u] = Piece<T>::load(x + (at < nvec ? at : nvec - 1) * V);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float v[V];
+                Piece<T>::unpack(raw[u], v);
+                const bool in = j + u * NT < nvec;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = in ? v[e] : -INFINITY;
+                if (j - tid + u * NT < nvec) add_scores<ENT>(s, v, a.c2);
+            }
+        }
+        if (rem) {
+            const float v[1] = {tid < rem ? to_f32(x[nvec * V + tid]) : -INFINITY};
+            add_scores<ENT>(s, v, a.c2);
+        }
+        const float m = s.m;
+        s = group_sums<NW, ENT>(s, a.c2, scratch[group]);
+        if (a.splits == 1) {
+            row_answer<T, NT, DISTILL>(a, r, row, s, tid);
+        } else if (tid == 0) {
+            a.part[unit] = make_float4(s.m, s.S, s.W, 0.f);
+        }
+        if constexpr (TOP) {
+            const int got = best_scores<T, NW>(x, n, (uint32_t)from, m, a.top, tid, top_scratch[group]);
+            write_best<T, NT>(a, r, row, s, top_scratch[group].key, got, a.splits == 1 ? nullptr : a.keys + unit * a.top, tid);
+        }
+        group_sync<NW>();                             // the scratch is free again
+    }
+}
+
+// a row's slices together: thread t holds slice t, its keys are in order
+template <typename T, bool ENT, bool TOP, bool DISTILL>
+__global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
+    __shared__ float scratch[3 * SC_NW];
+    __shared__ uint64_t buf[TOP ? SC_MAX_TOP * SC_MAX_TOP : 1];
+    __shared__ uint64_t heads[TOP ? SC_TPB : 1];
+    __shared__ uint64_t cut;
+    __shared__ int got;
+    const int tid = threadIdx.x;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = row_ptr<T>(a.x, r);
+        Sums s{-FLT_MAX, 0.f, 0.f};
+        if (tid < a.splits) {
+            const float4 p = a.part[r * a.splits + tid];
+            s = Sums{p.x, p.y, p.z};
+        }
+        s = group_sums<SC_NW, ENT>(s, a.c2, scratch);
+        row_answer<T, SC_TPB, DISTILL>(a, r, x, s, tid);
+        if constexpr (TOP) {
+            const uint64_t* keys = a.keys + (r * a.splits + tid) * a.top;
+            const uint64_t head = tid < a.splits ? keys[0] : 0;
+            heads[tid] = head;
+            if (tid == 0) {
+                cut = 1;
+                got = 0;
+            }
+            __syncthreads();
+            if (head) {                               // the top-th best of the slices' best keys is a bound for all
+                int rank = 0;
+                for (int i = 0; i < a.splits; ++i) rank += heads[i] > head ? 1 : 0;
+                if (rank == a.top - 1) cut = head;
+            }
+            __syncthreads();
+            if (head) {
+                for (int i = 0; i < a.top; ++i) {
+                    const uint64_t k = keys[i];
+                    if (k < cut) break;
+                    buf[atomicAdd(&got, 1)] = k;
+                }
+            }
+            __syncthreads();
+            write_best<T, SC_TPB>(a, r, x, s, buf, got, nullptr, tid);
+        }
+        __syncthreads();
+    }
+}
+
+// Slices of a row.  Rows alone fill the chip (8 blocks of 256 threads on each of 256 units) from 2048 on; fewer are cut into
+// slices of at least 4096 scores, at most one for each thread of the kernel that joins them.
+static int score_splits(int64_t rows, int64_t c) {
+    if (rows >= 2048 || c < 8192) return 1;
+    int64_t n = (2048 + rows - 1) / (rows < 1 ? 1 : rows);
+    if (n > c / 4096) n = c / 4096;
+    if (n > SC_TPB) n = SC_TPB;
+    return (int)(n < 1 ? 1 : n);
+}
+
+static int64_t score_ws(int64_t rows, int64_t c, int top) {
+    const int64_t splits = score_splits(rows, c);
+    return splits == 1 ? 0 : rows * splits * (16 + (int64_t)top * 8);
+}
+
+template <typename T, bool ENT, bool TOP, bool DISTILL>
+static int launch_score_fwd(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+    a.splits = score_splits(a.rows, a.c);
+    a.per = a.splits == 1 ? a.c : ((a.c + a.splits - 1) / a.splits + 63) / 64 * 64;
+    if (a.splits > 1) {
+        if (!ws || ws_bytes < score_ws(a.rows, a.c, a.top)) return ARMNET_ERR_BAD_ARG;
+        a.splits = (int)((a.c + a.per - 1) / a.per);                 // rounding up may leave the last slices empty
+        a.part = (float4*)ws;
+        a.keys = (uint64_t*)(a.part + a.rows * a.splits);
+    }
+    // a wave a row as long as its lanes hold the row in one go
+    if (a.c <= WAVE * Piece<T>::N * SC_UNROLL)
+        score_fwd_kernel<T, 1, ENT, TOP, DISTILL><<<row_grid((a.rows + 3) / 4), SC_TPB, 0, st>>>(a);
+    else
+        score_fwd_kernel<T, SC_NW, ENT, TOP, DISTILL><<<row_grid(a.rows * a.splits), SC_TPB, 0, st>>>(a);
+    ARMNET_LAUNCH_CHECK();
+    if (a.splits > 1) {
+        score_join_kernel<T, ENT, TOP, DISTILL><<<row_grid(a.rows), SC_TPB, 0, st>>>(a);
+        ARMNET_LAUNCH_CHECK();
+    }
+    return ARMNET_OK;
+}
+
+template <typename T>
+static int launch_scores(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+    if (a.entropy) return a.top ? launch_score_fwd<T, true, true, false>(a, ws, ws_bytes, st) : launch_score_fwd<T, true, false, false>(a, ws, ws_bytes, st);
+    return a.top ? launch_score_fwd<T, false, true, false>(a, ws, ws_bytes, st) : launch_score_fwd<T, false, false, false>(a, ws, ws_bytes, st);
 }
 
 // one row: p and its part of the gradient everywhere, then the listed ids' values again with what they add
@@ -274,7 +629,7 @@ extern "C" {
 
 int64_t armnet_score_ws_bytes(int64_t rows, int64_t c, int top) {
     if (rows < 0 || c <= 0 || top < 0) return -1;
-    return 0;
+    return score_ws(rows, c, top);
 }
 
 int armnet_score_logprobs_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
@@ -290,9 +645,7 @@ int armnet_score_logprobs_fwd(int64_t rows, int64_t inner, int64_t outer_stride,
     if ((n_ids > 0 && !logp) || (top > 0 && (!top_logp || !top_ids))) return ARMNET_ERR_BAD_ARG;
     a.logp = logp; a.entropy = entropy; a.top = top; a.top_logp = top_logp; a.top_ids = top_ids; a.stats = stats;
     a.id_status = id_status;
-    ARMNET_ROW_TYPE(x_type, T, (score_fwd_kernel<T><<<row_grid(rows), SC_TPB, 0, (hipStream_t)stream>>>(a)));
-    ARMNET_LAUNCH_CHECK();
-    return ARMNET_OK;
+    ARMNET_ROW_TYPE(x_type, T, return launch_scores<T>(a, workspace, ws_bytes, (hipStream_t)stream));
 }
 
 int armnet_score_logprobs_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
@@ -321,9 +674,7 @@ int armnet_distill_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_
     if (rows == 0) return ARMNET_OK;
     if (!teacher || !loss) return ARMNET_ERR_BAD_ARG;
     a.teacher = teacher; a.t_type = t_type; a.loss = loss; a.stats = stats; a.id_status = id_status;
-    ARMNET_ROW_TYPE(x_type, T, (distill_fwd_kernel<T><<<row_grid(rows), SC_TPB, 0, (hipStream_t)stream>>>(a)));
-    ARMNET_LAUNCH_CHECK();
-    return ARMNET_OK;
+    ARMNET_ROW_TYPE(x_type, T, return (launch_score_fwd<T, false, false, true>(a, workspace, ws_bytes, (hipStream_t)stream)));
 }
 
 int armnet_distill_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,

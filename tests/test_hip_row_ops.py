@@ -211,6 +211,21 @@ def test_alternatives_with_ties(c, dtype):
     check_scores(one, None, 1.0, min(c, 24))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_alternatives_in_a_pattern(dtype):
+    """the large scores recur at a fixed distance: a few threads meet all of them"""
+    c = 300001
+    n = 128 // torch.finfo(dtype).bits
+    at = torch.arange(c)
+    for period in (1024, 2048, 4096, 64 * n):
+        x = torch.randint(-50, 0, (2, c), generator=gen()).float()
+        big = (at % period) < n
+        x[0, big] = torch.arange(int(big.sum())).float() % 1000 / 4
+        x[1, big] = 7.0
+        for top in (1, 9, 64):
+            check_scores(x.to(dtype), None, 1.0, top)
+
+
 def score_gradients(x, ids, t, g, gh, dtype, got):
     dx, size = scores_grad_ref(x, ids, t, g, gh)
     n = 2 * chain(x.shape[-1]) + 4 * z_size(x, t) + 16
