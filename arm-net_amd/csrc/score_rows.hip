@@ -547,64 +547,143 @@ static int launch_scores(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
     return a.top ? launch_score_fwd<T, false, true, false>(a, ws, ws_bytes, st) : launch_score_fwd<T, false, false, false>(a, ws, ws_bytes, st);
 }
 
-// one row: p and its part of the gradient everywhere, then the listed ids' values again with what they add
-template <typename T, bool DISTILL>
+// The gradient of a slice of a row: p's part of it everywhere, then the listed ids' values again with what they add.  The first
+// slot of an id adds up all of them in order, so nothing depends on who comes first.  NW waves a slice; NW = 1: four rows a block.
+// List of a group in LDS: n4 ids (padded with -1 to whole fours), then n4 addends.
+template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
-    __shared__ float scratch[SC_NW];
-    __shared__ int32_t s_id[SC_MAX_IDS];
-    __shared__ float s_g[SC_MAX_IDS];
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* x = row_ptr<T>(a.x, r);
-        T* dx = (T*)a.dx + r * a.c;
+    constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
+    extern __shared__ int4 lists[];
+    const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1), lane = tid & (WAVE - 1);
+    const int n4 = (a.n_ids + 3) & ~3;
+    int32_t* s_id = (int32_t*)lists + group * 2 * n4;
+    float* s_g = (float*)(s_id + n4);
+    const int64_t units = a.rows * a.splits;
+    for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
+        const int64_t r = a.splits == 1 ? unit : unit / a.splits;
+        const int from = (int)((unit - r * a.splits) * a.per);
+        const int n = (int)(a.per < a.c - from ? a.per : a.c - from);
+        const int nvec = n / V, rem = n - nvec * V;
+        const T* x = row_ptr<T>(a.x, r) + from;
+        T* dx = (T*)a.dx + r * a.c + from;
         const float m = a.stats[(DISTILL ? 4 : 2) * r], l2 = a.stats[(DISTILL ? 4 : 2) * r + 1];
+        const float mt = DISTILL ? a.stats[4 * r + 2] : 0.f, lt = DISTILL ? a.stats[4 * r + 3] : 0.f;
         const bool none = l2 == INFINITY;
-        __syncthreads();                                // the row before is done with s_id, s_g
+        group_sync<NW>();                               // the slice before is done with the list
         float sum = 0.f;
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
-            const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
-            const bool in = id >= 0 && id < a.c && !none;
+        for (int k0 = 0; k0 < n4; k0 += WAVE) {         // every wave adds up the whole list, each keeps its share of it
+            const int k = k0 + lane;
+            int32_t at = -1;
             float g = 0.f;
-            if (DISTILL) {
-                if (id >= 0) g = exp2f((load_any(a.teacher, a.t_type, r * a.n_ids + k) - a.stats[4 * r + 2]) * a.c2 - a.stats[4 * r + 3]);
-            } else if (in && a.g_logp) {
-                g = a.g_logp[r * a.n_ids + k];
-                sum += g;
+            if (k < a.n_ids) {
+                const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                const bool in = id >= 0 && id < a.c && !none;
+                if (DISTILL) {
+                    if (in) g = exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2 - lt);
+                } else if (in && a.g_logp) {
+                    g = a.g_logp[r * a.n_ids + k];
+                    sum += g;
+                }
+                if (in && id >= from && id < from + n) at = (int32_t)id - from;
             }
-            s_id[k] = in ? (int32_t)id : -1;
-            s_g[k] = g;
+            if (k < n4 && (k0 / WAVE) % NW == tid / WAVE) {
+                s_id[k] = at;
+                s_g[k] = g;
+            }
         }
-        // dx = A p + B p (log2 p + H2) + (the listed ids) * u
+        // dx = p (A + B (log2 p + H2)) + u * (what the listed ids add)
         float A, B = 0.f, H2 = 0.f, u;
         if (DISTILL) {
             u = -a.g_logp[r] * a.t;
-            const float lt = a.stats[4 * r + 3];
-            A = lt == INFINITY ? 0.f : -u + (lt - lt);     // a teacher without a distribution (NaN) has no gradient either
+            A = lt == INFINITY ? 0.f : -u + (lt - lt);  // a teacher without a distribution (NaN) has no gradient either
         } else {
-            A = -block_sum<SC_NW>(sum, scratch) / a.t;
-            u = 1.f / a.t;
-            if (a.g_entropy) {
-                B = -a.g_entropy[r] * LN2 / a.t;
+            A = -wave_sum(sum) * a.rt;
+            u = a.rt;
+            if (ENT) {
+                B = -a.g_entropy[r] * LN2 * a.rt;
                 H2 = a.entropy[r] / LN2;
             }
         }
-        __syncthreads();
         auto base = [&](float xv) {
-            const float lp = (xv - m) * a.c2 - l2;
-            return exp2f(lp) * fmaf(B, fmaxf(lp, Z_FLOOR) + H2, A);
+            const float lp = fmaf(xv - m, a.c2, -l2);
+            const float p = exp2_raw(lp);
+            return ENT ? p * fmaf(B, fmaxf(lp, Z_FLOOR) + H2, A) : p * A;
         };
-        for (int i = threadIdx.x; i < a.c; i += SC_TPB) dx[i] = from_f32<T>(base(to_f32(x[i])));
-        __syncthreads();
-        for (int k = threadIdx.x; k < a.n_ids; k += SC_TPB) {
+        int64_t j = tid;
+        for (; j - tid + U * NT <= nvec; j += U * NT) {
+            u32x4 raw[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) raw[i] = Piece<T>::load(x + (j + i * NT) * V);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                float v[V];
+                Piece<T>::unpack(raw[i], v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = base(v[e]);
+                Piece<T>::store(dx + (j + i * NT) * V, Piece<T>::pack(v));
+            }
+        }
+        if (j - tid < nvec) {
+            u32x4 raw[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) raw[i] = Piece<T>::load(x + (j + i * NT < nvec ? j + i * NT : nvec - 1) * V);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (j + i * NT < nvec) {
+                    float v[V];
+                    Piece<T>::unpack(raw[i], v);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] = base(v[e]);
+                    Piece<T>::store(dx + (j + i * NT) * V, Piece<T>::pack(v));
+                }
+            }
+        }
+        if (tid < rem) dx[nvec * V + tid] = from_f32<T>(base(to_f32(x[nvec * V + tid])));
+        if (a.n_ids == 0) continue;
+        // the list is complete, and the stores above come before the ones below
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        group_sync<NW>();
+        for (int k = tid; k < a.n_ids; k += NT) {
             const int32_t id = s_id[k];
             if (id < 0) continue;
             float g = s_g[k];
-            bool first = true;
-            for (int j = 0; j < k; ++j) first = first && s_id[j] != id;
-            if (!first) continue;                       // the first slot of an id adds up all of them, in order
-            for (int j = k + 1; j < a.n_ids; ++j) g += s_id[j] == id ? s_g[j] : 0.f;
+            int same = 0;
+            for (int i = 0; i < n4; i += 4) {
+                const int4 o = *(const int4*)(s_id + i);
+                same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+            }
+            if (same > 1) {
+                bool first = true;
+                for (int i = 0; i < k; ++i) first = first && s_id[i] != id;
+                if (!first) continue;
+                for (int i = k + 1; i < a.n_ids; ++i) g += s_id[i] == id ? s_g[i] : 0.f;
+            }
             dx[id] = from_f32<T>(fmaf(g, u, base(to_f32(x[id]))));
         }
     }
+}
+
+template <typename T, bool ENT, bool DISTILL>
+static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
+    const bool narrow = a.c <= WAVE * Piece<T>::N * SC_UNROLL;
+    // slices of at most 65536 scores; few rows: down to what a block's threads load at once
+    const int64_t at_once = SC_TPB * Piece<T>::N * SC_UNROLL;
+    int64_t splits = (a.c + 65535) / 65536;
+    if (a.rows < 2048) {
+        int64_t want = (2048 + a.rows - 1) / a.rows;
+        if (want > (a.c + at_once - 1) / at_once) want = (a.c + at_once - 1) / at_once;
+        if (want > splits) splits = want;
+    }
+    if (narrow) splits = 1;
+    a.per = splits == 1 ? a.c : ((a.c + splits - 1) / splits + 63) / 64 * 64;
+    a.splits = (int)((a.c + a.per - 1) / a.per);
+    const size_t list = (size_t)((a.n_ids + 3) & ~3) * 8;
+    if (narrow)
+        score_bwd_kernel<T, 1, ENT, DISTILL><<<row_grid((a.rows + 3) / 4), SC_TPB, 4 * list, st>>>(a);
+    else
+        score_bwd_kernel<T, SC_NW, ENT, DISTILL><<<row_grid(a.rows * a.splits), SC_TPB, list, st>>>(a);
+    ARMNET_LAUNCH_CHECK();
+    return ARMNET_OK;
 }
 
 static int score_common(ScoreArgs& a, int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c,
@@ -658,9 +737,8 @@ int armnet_score_logprobs_bwd(int64_t rows, int64_t inner, int64_t outer_stride,
     if (rows == 0) return ARMNET_OK;
     if (!stats || !dx || (g_entropy && !entropy)) return ARMNET_ERR_BAD_ARG;
     a.stats = (float*)stats; a.entropy = (float*)entropy; a.g_logp = g_logp; a.g_entropy = g_entropy; a.dx = dx;
-    ARMNET_ROW_TYPE(x_type, T, (score_bwd_kernel<T, false><<<row_grid(rows), SC_TPB, 0, (hipStream_t)stream>>>(a)));
-    ARMNET_LAUNCH_CHECK();
-    return ARMNET_OK;
+    hipStream_t st = (hipStream_t)stream;
+    ARMNET_ROW_TYPE(x_type, T, return g_entropy ? (launch_score_bwd<T, true, false>(a, st)) : (launch_score_bwd<T, false, false>(a, st)));
 }
 
 int armnet_distill_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
@@ -687,9 +765,7 @@ int armnet_distill_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_
     if (rows == 0) return ARMNET_OK;
     if (!teacher || !stats || !g_loss || !dx) return ARMNET_ERR_BAD_ARG;
     a.teacher = teacher; a.t_type = t_type; a.stats = (float*)stats; a.g_logp = g_loss; a.dx = dx;
-    ARMNET_ROW_TYPE(x_type, T, (score_bwd_kernel<T, true><<<row_grid(rows), SC_TPB, 0, (hipStream_t)stream>>>(a)));
-    ARMNET_LAUNCH_CHECK();
-    return ARMNET_OK;
+    ARMNET_ROW_TYPE(x_type, T, return (launch_score_bwd<T, false, true>(a, (hipStream_t)stream)));
 }
 
 }  // extern "C"
