@@ -112,7 +112,7 @@ def _wide(x):
 
 
 def layer_norm_fwd(x, weight, bias, eps):
-    """y, mean [.., 1], rstd [.., 1]"""
+    """y and the statistics [2, .., 1]: mean, 1 / standard deviation"""
     xw = _wide(x)
     mean = xw.mean(-1, keepdim=True)
     xc = xw - mean
@@ -122,10 +122,11 @@ def layer_norm_fwd(x, weight, bias, eps):
         y = y * _wide(weight)
     if bias is not None:
         y = y + _wide(bias)
-    return y.to(x.dtype), mean, rstd
+    return y.to(x.dtype), torch.stack((mean, rstd))
 
 
-def layer_norm_bwd(x, dy, weight, mean, rstd, need_dx, need_dw, need_db, p_dtype):
+def layer_norm_bwd(x, dy, weight, st, need_dx, need_dw, need_db, p_dtype):
+    mean, rstd = st
     dyw, h = _wide(dy), (_wide(x) - mean) * rstd
     g = dyw if weight is None else dyw * _wide(weight)
     dx = (rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))).to(x.dtype) if need_dx else None

@@ -713,135 +713,166 @@ def row_view(x):
     return x, x.numel() // d, 0, 0, d
 
 
-def _row_args(x, name):
-    """the leading arguments of a row call (address and all) and the tensor that has to stay alive through it"""
-    x, rows, inner, so, sr = row_view(x)
-    return x, (rows, inner, so, sr, x.shape[-1], row_type(x, name), x.data_ptr())
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _row_stream(dev):
+    """the current stream of device `dev`, as an address (these calls are short: the Stream object costs more than a launch)"""
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _on_its_device(fn):
+    """run `fn(x, ...)` with x's device as the current one (the library queries it); host tensors raise"""
+    def call(x, *args):
+        if not x.is_cuda:
+            raise ArmnetNativeError(f"expected a tensor on the HIP device, got one on {x.device} (no CPU fallback)")
+        dev = x.get_device()
+        if dev == torch.cuda.current_device():
+            return fn(dev, x, *args)
+        with torch.cuda.device(dev):
+            return fn(dev, x, *args)
+    call.__name__, call.__doc__ = fn.__name__, fn.__doc__
+    return call
 
 
 def _addr(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
-def _same_dense(t, shape, device, name, dtype=None):
-    if t is not None and (t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous()
-                          or (dtype is not None and t.dtype != dtype)):
-        raise ArmnetNativeError(f"{name}: expected a dense {list(shape)} tensor{'' if dtype is None else f' of {dtype}'} on "
-                                f"{device}, got {list(t.shape)} {t.dtype} on {t.device} (contiguous={t.is_contiguous()})")
+def _dense(t, n, dev, name, dtype):
+    """`t` (or None) is n adjacent elements of dtype on device dev"""
+    if t is not None and not (t.is_contiguous() and t.numel() == n and t.dtype == dtype and t.get_device() == dev):
+        raise ArmnetNativeError(f"{name}: expected {n} adjacent elements of {dtype} on device {dev}, got {list(t.shape)} "
+                                f"{t.dtype} on {t.device} (contiguous={t.is_contiguous()})")
 
 
-def _row_device(x):
-    if not x.is_cuda:
-        raise ArmnetNativeError(f"expected a tensor on the HIP device, got one on {x.device} (no CPU fallback)")
-    return torch.cuda.device(x.device)
+def _like(x):
+    """a new dense tensor of x's shape, type and device"""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
 
 
-def layer_norm_fwd(x, weight, bias, eps, stats):
-    """armnet_layer_norm_fwd: y, and with `stats` the rows' mean and 1 / standard deviation (else None, None)"""
+@_on_its_device
+def layer_norm_fwd(dev, x, weight, bias, eps, stats):
+    """armnet_layer_norm_fwd(x, weight, bias, eps, stats): (y, statistics [2, rows] for the backward or None)"""
+    x, rows, inner, so, sr = row_view(x)
+    d = x.shape[-1]
+    p = weight if weight is not None else bias
+    if p is not None:
+        _dense(weight, d, dev, "weight", p.dtype)
+        _dense(bias, d, dev, "bias", p.dtype)
+    y = _like(x)
+    st = mean = rstd = None
+    if stats:
+        st = torch.empty((2, rows), device=x.device, dtype=torch.float32)
+        mean = st.data_ptr()
+        rstd = mean + 4 * rows
+    if rows:
+        check(load().armnet_layer_norm_fwd(rows, inner, so, sr, d, row_type(x, "x"), x.data_ptr(),
+                                           F32 if p is None else row_type(p, "weight"), _addr(weight), _addr(bias), eps,
+                                           y.data_ptr(), mean, rstd, _row_stream(dev)))
+    return y, st
+
+
+@_on_its_device
+def layer_norm_bwd(dev, x, dy, weight, st, need_dx, need_dw, need_db, p_dtype):
+    """armnet_layer_norm_bwd(x, dy, weight, statistics, ...): (dx, dweight, dbias), None where not needed; the parameters'
+    gradients in p_dtype"""
     lib = load()
-    with _row_device(x):
-        x, view = _row_args(x, "x")
-        p = weight if weight is not None else bias
-        wt = F32 if p is None else row_type(p, "weight")
-        for t, name in ((weight, "weight"), (bias, "bias")):
-            _same_dense(t, (x.shape[-1],), x.device, name, None if p is None else p.dtype)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        mean, rstd = torch.empty(2, view[0], device=x.device, dtype=torch.float32) if stats else (None, None)
-        if view[0]:
-            check(lib.armnet_layer_norm_fwd(*view, wt, _addr(weight), _addr(bias), eps, y.data_ptr(), _addr(mean), _addr(rstd),
-                                            torch.cuda.current_stream().cuda_stream))
-    return y, mean, rstd
-
-
-def layer_norm_bwd(x, dy, weight, mean, rstd, need_dx, need_dw, need_db, p_dtype):
-    """armnet_layer_norm_bwd: (dx, dweight, dbias), None where not needed; the parameters' gradients in p_dtype"""
-    lib = load()
-    with _row_device(x):
-        x, view = _row_args(x, "x")
-        dy = dy.contiguous()
-        _same_dense(dy, x.shape, x.device, "dy", x.dtype)
-        d, dev = x.shape[-1], x.device
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need_dx else None
-        dw = torch.empty(d, device=dev, dtype=p_dtype) if need_dw else None
-        db = torch.empty(d, device=dev, dtype=p_dtype) if need_db else None
-        ws, n = None, 0
-        if need_dw or need_db:
-            n = lib.armnet_layer_norm_bwd_ws_bytes(view[0], d)
-            ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        check(lib.armnet_layer_norm_bwd(*view, dy.data_ptr(), _ROW_TYPES[p_dtype] if p_dtype is not None else F32, _addr(weight),
-                                        _addr(mean), _addr(rstd), _addr(dx), _addr(dw), _addr(db), _addr(ws), n,
-                                        torch.cuda.current_stream().cuda_stream))
+    x, rows, inner, so, sr = row_view(x)
+    d = x.shape[-1]
+    dy = dy.contiguous()
+    _dense(dy, rows * d, dev, "dy", x.dtype)
+    dx = _like(x) if need_dx else None
+    dw = torch.empty((d,), device=x.device, dtype=p_dtype) if need_dw else None
+    db = torch.empty((d,), device=x.device, dtype=p_dtype) if need_db else None
+    n = lib.armnet_layer_norm_bwd_ws_bytes(rows, d) if need_dw or need_db else 0
+    ws = torch.empty((n,), device=x.device, dtype=torch.uint8) if n else None
+    mean = st.data_ptr()
+    check(lib.armnet_layer_norm_bwd(rows, inner, so, sr, d, row_type(x, "x"), x.data_ptr(), dy.data_ptr(),
+                                    F32 if p_dtype is None else _ROW_TYPES[p_dtype], _addr(weight), mean, mean + 4 * rows,
+                                    _addr(dx), _addr(dw), _addr(db), _addr(ws), n, _row_stream(dev)))
     return dx, dw, db
 
 
-def score_logprobs_fwd(X, ids, temperature, top_k, entropy, stats, id_status=None):
-    """armnet_score_logprobs_fwd: ids [.., n_ids] dense or None -> (logp, entropy, top_logp, top_ids, stats), None where not
-    asked for"""
+def _score_ids(ids, lead, dev, name):
+    """(ids of a row, their type): `ids` [.., n] dense beside rows of the shape `lead`"""
+    if ids is None:
+        return 0, ID_I64
+    if tuple(ids.shape[:-1]) != tuple(lead) or not ids.is_contiguous() or ids.get_device() != dev:
+        raise ArmnetNativeError(f"{name}: expected a dense {list(lead) + ['n']} tensor on device {dev}, got {list(ids.shape)} on "
+                                f"{ids.device} (contiguous={ids.is_contiguous()})")
+    return ids.shape[-1], _id_type(ids)
+
+
+@_on_its_device
+def score_logprobs_fwd(dev, X, ids, temperature, top_k, entropy, stats, id_status=None):
+    """armnet_score_logprobs_fwd(X, ids, temperature, top_k, entropy, stats, id_status): ids [.., n_ids] dense or None ->
+    (logp, entropy, top_logp, top_ids, stats), None where not asked for"""
     lib = load()
-    with _row_device(X):
-        X, view = _row_args(X, "X")
-        lead, dev = X.shape[:-1], X.device
-        n_ids = 0 if ids is None else ids.shape[-1]
-        if ids is not None:
-            _same_dense(ids, lead + (n_ids,), dev, "ids")
-        new = lambda *shape, dtype=torch.float32: torch.empty(*shape, device=dev, dtype=dtype)   # noqa: E731
-        logp = None if ids is None else new(lead + (n_ids,))
-        ent = new(lead) if entropy else None
-        tl, ti = (new(lead + (top_k,)), new(lead + (top_k,), dtype=torch.int64)) if top_k else (None, None)
-        st = new(view[0], 2) if stats else None
-        n = lib.armnet_score_ws_bytes(view[0], view[4], top_k)
-        ws = new(n, dtype=torch.uint8) if n > 0 else None
-        if view[0]:
-            check(lib.armnet_score_logprobs_fwd(*view, temperature, n_ids, _addr(ids), ID_I64 if ids is None else _id_type(ids),
-                                                top_k, _addr(logp), _addr(ent), _addr(tl), _addr(ti), _addr(st), _addr(ws), n,
-                                                _addr(id_status), torch.cuda.current_stream().cuda_stream))
+    X, rows, inner, so, sr = row_view(X)
+    c, lead, where, f32 = X.shape[-1], X.shape[:-1], X.device, torch.float32
+    n_ids, id_type = _score_ids(ids, lead, dev, "ids")
+    logp = None if ids is None else torch.empty(ids.shape, device=where, dtype=f32)
+    ent = torch.empty(lead, device=where, dtype=f32) if entropy else None
+    tl = ti = None
+    if top_k:
+        tl = torch.empty(lead + (top_k,), device=where, dtype=f32)
+        ti = torch.empty(lead + (top_k,), device=where, dtype=torch.int64)
+    st = torch.empty((rows, 2), device=where, dtype=f32) if stats else None
+    n = lib.armnet_score_ws_bytes(rows, c, top_k)
+    ws = torch.empty((n,), device=where, dtype=torch.uint8) if n > 0 else None
+    if rows:
+        check(lib.armnet_score_logprobs_fwd(rows, inner, so, sr, c, row_type(X, "X"), X.data_ptr(), temperature, n_ids, _addr(ids),
+                                            id_type, top_k, _addr(logp), _addr(ent), _addr(tl), _addr(ti), _addr(st), _addr(ws),
+                                            n, _addr(id_status), _row_stream(dev)))
     return logp, ent, tl, ti, st
 
 
-def score_logprobs_bwd(X, ids, temperature, stats, entropy, g_logp, g_entropy):
-    """armnet_score_logprobs_bwd: the gradient of X (dense) from those of logp and entropy (either may be None)"""
-    lib = load()
-    with _row_device(X):
-        X, view = _row_args(X, "X")
-        dx = torch.empty(X.shape, device=X.device, dtype=X.dtype)
-        n_ids = 0 if ids is None else ids.shape[-1]
-        _same_dense(g_logp, () if ids is None else ids.shape, X.device, "the gradient of logp", torch.float32)
-        _same_dense(g_entropy, X.shape[:-1], X.device, "the gradient of entropy", torch.float32)
-        if view[0]:
-            check(lib.armnet_score_logprobs_bwd(*view, temperature, n_ids, _addr(ids), ID_I64 if ids is None else _id_type(ids),
-                                                stats.data_ptr(), _addr(entropy), _addr(g_logp), _addr(g_entropy), dx.data_ptr(),
-                                                torch.cuda.current_stream().cuda_stream))
+@_on_its_device
+def score_logprobs_bwd(dev, X, ids, temperature, stats, entropy, g_logp, g_entropy):
+    """armnet_score_logprobs_bwd(X, ids, temperature, stats, entropy, g_logp, g_entropy): the gradient of X (dense) from those of
+    logp and entropy (either may be None)"""
+    X, rows, inner, so, sr = row_view(X)
+    n_ids, id_type = _score_ids(ids, X.shape[:-1], dev, "ids")
+    _dense(g_logp, rows * n_ids, dev, "the gradient of logp", torch.float32)
+    _dense(g_entropy, rows, dev, "the gradient of entropy", torch.float32)
+    dx = _like(X)
+    if rows:
+        check(load().armnet_score_logprobs_bwd(rows, inner, so, sr, X.shape[-1], row_type(X, "X"), X.data_ptr(), temperature, n_ids,
+                                               _addr(ids), id_type, stats.data_ptr(), _addr(entropy), _addr(g_logp),
+                                               _addr(g_entropy), dx.data_ptr(), _row_stream(dev)))
     return dx
 
 
-def distill_fwd(X, ids, teacher, temperature, stats, id_status=None):
-    """armnet_distill_fwd: (loss per row, stats for the backward or None); ids and teacher [.., k] dense"""
+@_on_its_device
+def distill_fwd(dev, X, ids, teacher, temperature, stats, id_status=None):
+    """armnet_distill_fwd(X, ids, teacher, temperature, stats, id_status): (loss per row, stats for the backward or None); ids and
+    teacher [.., k] dense"""
     lib = load()
-    with _row_device(X):
-        X, view = _row_args(X, "X")
-        lead, dev, k = X.shape[:-1], X.device, ids.shape[-1]
-        _same_dense(ids, lead + (k,), dev, "top_ids")
-        _same_dense(teacher, lead + (k,), dev, "top_scores")
-        loss = torch.empty(lead, device=dev, dtype=torch.float32)
-        st = torch.empty(view[0], 4, device=dev, dtype=torch.float32) if stats else None
-        n = lib.armnet_score_ws_bytes(view[0], view[4], 0)
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
-        if view[0]:
-            check(lib.armnet_distill_fwd(*view, temperature, k, ids.data_ptr(), _id_type(ids), row_type(teacher, "top_scores"),
-                                         teacher.data_ptr(), loss.data_ptr(), _addr(st), _addr(ws), n, _addr(id_status),
-                                         torch.cuda.current_stream().cuda_stream))
+    X, rows, inner, so, sr = row_view(X)
+    c, lead = X.shape[-1], X.shape[:-1]
+    k, id_type = _score_ids(ids, lead, dev, "top_ids")
+    _dense(teacher, rows * k, dev, "top_scores", teacher.dtype)
+    loss = torch.empty(lead, device=X.device, dtype=torch.float32)
+    st = torch.empty((rows, 4), device=X.device, dtype=torch.float32) if stats else None
+    n = lib.armnet_score_ws_bytes(rows, c, 0)
+    ws = torch.empty((n,), device=X.device, dtype=torch.uint8) if n > 0 else None
+    if rows:
+        check(lib.armnet_distill_fwd(rows, inner, so, sr, c, row_type(X, "X"), X.data_ptr(), temperature, k, ids.data_ptr(), id_type,
+                                     row_type(teacher, "top_scores"), teacher.data_ptr(), loss.data_ptr(), _addr(st), _addr(ws), n,
+                                     _addr(id_status), _row_stream(dev)))
     return loss, st
 
 
-def distill_bwd(X, ids, teacher, temperature, stats, g_loss):
-    """armnet_distill_bwd: the gradient of X (dense) from that of the rows' losses"""
-    lib = load()
-    with _row_device(X):
-        X, view = _row_args(X, "X")
-        _same_dense(g_loss, X.shape[:-1], X.device, "the gradient of the loss", torch.float32)
-        dx = torch.empty(X.shape, device=X.device, dtype=X.dtype)
-        if view[0]:
-            check(lib.armnet_distill_bwd(*view, temperature, ids.shape[-1], ids.data_ptr(), _id_type(ids),
-                                         row_type(teacher, "top_scores"), teacher.data_ptr(), stats.data_ptr(),
-                                         g_loss.data_ptr(), dx.data_ptr(), torch.cuda.current_stream().cuda_stream))
+@_on_its_device
+def distill_bwd(dev, X, ids, teacher, temperature, stats, g_loss):
+    """armnet_distill_bwd(X, ids, teacher, temperature, stats, g_loss): the gradient of X (dense) from that of the rows' losses"""
+    X, rows, inner, so, sr = row_view(X)
+    k, id_type = _score_ids(ids, X.shape[:-1], dev, "top_ids")
+    _dense(g_loss, rows, dev, "the gradient of the loss", torch.float32)
+    dx = _like(X)
+    if rows:
+        check(load().armnet_distill_bwd(rows, inner, so, sr, X.shape[-1], row_type(X, "X"), X.data_ptr(), temperature, k,
+                                        ids.data_ptr(), id_type, row_type(teacher, "top_scores"), teacher.data_ptr(),
+                                        stats.data_ptr(), g_loss.data_ptr(), dx.data_ptr(), _row_stream(dev)))
     return dx

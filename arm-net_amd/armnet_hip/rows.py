@@ -18,6 +18,16 @@ from .block import IdStatus, _id_mode
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _once(backward):
+    """A backward that is not itself differentiable.  Most backwards run with gradients off, where there is nothing to mark; they
+    run on the engine's own thread, where every Python step costs several times what it costs the caller."""
+    marked = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return marked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 def _place(what, first, *others):
     """True on the device, False on the host; tensors in different places raise"""
     for name, t in others:
@@ -44,21 +54,20 @@ def _temperature(t):
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        if x.is_cuda:
-            y, mean, rstd = native.layer_norm_fwd(x, weight, bias, eps, True)
-        else:
-            y, mean, rstd = host_ops.layer_norm_fwd(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, st = native.layer_norm_fwd(x, weight, bias, eps, True) if x.is_cuda else host_ops.layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, st)
         p = weight if weight is not None else bias
         ctx.p_dtype = None if p is None else p.dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, st = ctx.saved_tensors
+        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
         bwd = native.layer_norm_bwd if x.is_cuda else host_ops.layer_norm_bwd
-        return bwd(x, dy, weight, mean, rstd, *ctx.needs_input_grad[:3], ctx.p_dtype) + (None,)
+        dx, dw, db = bwd(x, dy, weight, st, need_dx, need_dw, need_db, ctx.p_dtype)
+        return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -126,7 +135,7 @@ class _ScoreLogprobsFn(torch.autograd.Function):
         return logp, ent, tl, ti
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g_logp, g_entropy, _tl, _ti):
         X, ids, st, ent = ctx.saved_tensors
         if g_logp is None and g_entropy is None:
@@ -223,7 +232,7 @@ class _DistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         X, ids, teacher, st = ctx.saved_tensors
         g = g.contiguous()

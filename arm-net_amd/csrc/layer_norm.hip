@@ -32,7 +32,8 @@ struct NormArgs {
     float* mean;           // [rows]
     float* rstd;           // [rows]
     // backward
-    float* partial;        // [blocks, 2, d] or null: no parameter gradients
+    bool params;           // the parameters' gradients are wanted
+    float* partial;        // [blocks, 2, d], for more than one block
     void* dweight;         // [d] or null
     void* dbias;
     int blocks;
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
         }
         cur = next;
     }
-    if (!a.partial) return;
+    if (!a.params) return;
     int share = group;
     if constexpr (LPR < WAVE) {
 #pragma unroll
@@ -472,7 +473,8 @@ int armnet_layer_norm_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int
 int64_t armnet_layer_norm_bwd_ws_bytes(int64_t rows, int64_t d) {
     if (rows < 0 || d <= 0) return -1;
     const int n4 = norm_blocks(rows, d, 4), n8 = norm_blocks(rows, d, 8);
-    return (int64_t)(n4 > n8 ? n4 : n8) * 2 * d * 4;
+    const int64_t n = n4 > n8 ? n4 : n8;
+    return n == 1 && d <= LN_MAX_D ? 0 : n * 2 * d * 4;              // one block writes the gradients by itself
 }
 
 int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t d, int x_type,
@@ -482,13 +484,13 @@ int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int
     if (rows >= ((int64_t)1 << 31) || d >= ((int64_t)1 << 31)) return ARMNET_ERR_UNSUPPORTED;
     if (rows > 0 && (!x || !dy || !mean || !rstd)) return ARMNET_ERR_BAD_ARG;
     const bool params = dweight || dbias;
-    if (params && rows > 0 && (!workspace || ws_bytes < armnet_layer_norm_bwd_ws_bytes(rows, d))) return ARMNET_ERR_BAD_ARG;
+    if (params && rows > 0 && (ws_bytes < armnet_layer_norm_bwd_ws_bytes(rows, d) || (ws_bytes > 0 && !workspace))) return ARMNET_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     NormArgs a{};
     a.rows = rows; a.d = (int)d;
     a.x = RowView{x, inner, outer_stride, row_stride};
     a.dy = dy; a.w_type = w_type; a.weight = weight; a.out = dx; a.mean = (float*)mean; a.rstd = (float*)rstd;
-    a.partial = params ? (float*)workspace : nullptr;
+    a.params = params; a.partial = (float*)workspace;
     a.dweight = dweight; a.dbias = dbias;
     a.blocks = norm_blocks(rows, d, x_type == ARMNET_F32 ? 4 : 8);
     if (rows > 0 && (dx || params)) {

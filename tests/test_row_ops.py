@@ -187,6 +187,8 @@ def test_empty_batches_on_host():
 # ---- the C entries -------------------------------------------------------------------------------------------------------
 
 def test_c_entries_check_their_arguments():
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: only where nothing can be launched")
     lib = native.load()
     bad, unsup, ok = native.ERR_BAD_ARG, native.ERR_UNSUPPORTED, native.OK
     P = 1 << 20                                                  # an address that is never used: no call below launches
@@ -203,7 +205,10 @@ def test_c_entries_check_their_arguments():
     assert fwd(*view(d=1 << 31), 0, None, None, 1e-5, P, None, None, None) == unsup
     assert fwd(*view(rows=0, x=None), 0, None, None, 1e-5, None, None, None, None) == ok
     bwd = lib.armnet_layer_norm_bwd
-    assert bwd(*view(), P, 0, None, P, P, P, P, None, None, 0, None) == bad    # parameter gradients without a workspace
+    need = lib.armnet_layer_norm_bwd_ws_bytes(100000, 8)                        # parameter gradients of many rows: a workspace
+    assert need > 0 and bwd(*view(rows=100000), P, 0, None, P, P, P, P, None, None, 0, None) == bad
+    assert bwd(*view(rows=100000), P, 0, None, P, P, P, P, None, P, need - 1, None) == bad
+    assert bwd(*view(rows=100000), P, 0, None, P, P, P, P, None, None, need, None) == bad
     assert bwd(*view(), None, 0, None, P, P, P, None, None, None, 0, None) == bad
     assert bwd(*view(rows=0, x=None), None, 0, None, None, None, None, None, None, None, 0, None) == ok
     assert lib.armnet_layer_norm_bwd_ws_bytes(-1, 8) == -1 and lib.armnet_layer_norm_bwd_ws_bytes(4, 0) == -1
