@@ -77,11 +77,27 @@ __device__ __forceinline__ uint64_t score_key(float v, uint32_t id) { return ((u
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }   // results below 2^-126 are 0
 
+template <int NW>
+__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* scratch) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        const uint64_t o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
+    __syncthreads();
+    if ((threadIdx.x & (WAVE - 1)) == 0) scratch[threadIdx.x / WAVE] = v;
+    __syncthreads();
+    uint64_t s = scratch[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) s = scratch[w] > s ? scratch[w] : s;
+    return s;
+}
+
 struct Sums {
     float m, S, W;             // largest score, sum of e^z, sum of e^z z2
 };
 
-// moves sums to another reference m' >= m
+// moves sums to another reference
 template <bool ENT>
 __device__ __forceinline__ void rebase(Sums& s, float m, float c2) {
     const float d = fmaxf((s.m - m) * c2, Z_FLOOR);
@@ -91,8 +107,9 @@ __device__ __forceinline__ void rebase(Sums& s, float m, float c2) {
     s.m = m;
 }
 
+// The largest score so far is the reference.  Returns the largest of these.
 template <bool ENT, int N>
-__device__ __forceinline__ void add_scores(Sums& s, const float (&v)[N], float c2) {
+__device__ __forceinline__ float add_scores(Sums& s, const float (&v)[N], float c2) {
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
@@ -107,7 +124,20 @@ __device__ __forceinline__ void add_scores(Sums& s, const float (&v)[N], float c
     }
     s.S += e0;
     if constexpr (ENT) s.W += w0;
+    return mx;
 }
+
+// the largest score of a thread, the batch of pieces it is in (by its first piece; -1: behind the last piece) and the largest score
+// of all other batches
+struct Peak {
+    float m1, m2;
+    int at;
+    __device__ __forceinline__ void add(float mx, int batch) {
+        at = mx > m1 ? batch : at;
+        m2 = __builtin_amdgcn_fmed3f(m1, m2, mx);
+        m1 = fmaxf(m1, mx);
+    }
+};
 
 // all threads' sums of a group, in every thread; scratch: 3 * NW floats of the group's own
 template <int NW, bool ENT>
@@ -139,12 +169,13 @@ __device__ __forceinline__ Sums group_sums(Sums s, float c2, float* scratch) {
     return s;
 }
 
-constexpr int SC_UNROLL = 4;             // pieces of 16 bytes in flight a thread
+constexpr int SC_UNROLL = 2;             // pieces of 16 bytes in flight a thread
 constexpr int SC_BUF = 512;              // candidates for the alternatives
+constexpr int SC_FEW = 128;              // so few scores are all candidates
 
 template <int NW>
 struct TopScratch {
-    uint64_t key[SC_BUF];
+    uint64_t key[SC_BUF + 8];
     int n, threads, first;
     uint32_t cut;
     int count[NW];
@@ -187,17 +218,27 @@ __device__ int count_from(const T* x, int n, float cut, int tid, TopScratch<NW>&
 }
 
 // The `top` best scores of a slice of n scores that begins at id `id0`, as keys in ts.key[0 .. result), unordered; the result is at
-// most SC_BUF and covers the best ones.  m: the largest score that this thread met; it owns the pieces tid, tid + NT, ...
+// most SC_BUF and covers the best ones.  pk: the peak of this thread, which owns the pieces tid, tid + NT, ...
 //
-// The top-th largest of the threads' maxima is a bound: at least `top` scores reach it, and few more do (for scores in no
-// particular order top + top^2 / 2 NT).  Only the pieces of the threads whose maximum reaches it are read again, a thread's
-// pieces by the 64 lanes of a wave.  Where more than SC_BUF scores reach the bound (ties, or scores that grow along the pieces
-// of one thread), the bound is raised by halving until it fits; if ties remain, the ones with the lowest ids are taken.
+// The top-th largest of the threads' largest scores is a bound: at least `top` scores reach it, and few more do (for scores in no
+// particular order about top + top^2 / 2 NT).  A thread whose largest score reaches it reads the batch that holds it again; the few
+// that have a second batch with such a score read all of theirs.  Where more than SC_BUF scores reach the bound (ties, or large
+// scores that recur at a fixed distance), it is raised by halving until they fit; if ties remain, the ones with the lowest ids are
+// taken.
 template <typename T, int NW>
-__device__ int best_scores(const T* x, int n, uint32_t id0, float m, int top, int tid, TopScratch<NW>& ts) {
-    constexpr int NT = NW * WAVE, V = Piece<T>::N;
+__device__ int best_scores(const T* x, int n, uint32_t id0, const Peak& pk, int top, int tid, TopScratch<NW>& ts) {
+    constexpr int NT = NW * WAVE, V = Piece<T>::N, U = SC_UNROLL;
+    const float m = pk.m1;
     const int lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int nvec = n / V, rem = n - nvec * V;
+    if (n <= SC_FEW) {                   // all of them; a masked one is below every other and has no value
+        for (int i = tid; i < n; i += NT) {
+            const float v = to_f32(x[i]);
+            ts.key[i] = v > -INFINITY ? score_key(v, id0 + i) : (uint64_t)~(id0 + i);
+        }
+        group_sync<NW>();
+        return n;
+    }
     float* maxima = (float*)ts.key;
     if constexpr (NW > 1) maxima[tid] = m;
     if (tid == 0) ts.n = ts.threads = 0;
@@ -214,38 +255,50 @@ __device__ int best_scores(const T* x, int n, uint32_t id0, float m, int top, in
         }
         uint32_t lo = value_key(-wave_max(-mn)), hi = value_key(wave_max(mx)) + 1;
         int reach = NT;
+        uint32_t mid = lo + 1;           // first: are there `top` threads at all above the least (those without a score)?
         while (hi - lo > 1 && reach > top + 8) {
-            const uint32_t mid = lo + (hi - lo) / 2;
             int c = 0;
 #pragma unroll
             for (int i = 0; i < NW; ++i) c += __popcll(__ballot(k[i] >= mid));
             if (c >= top) { lo = mid; reach = c; } else hi = mid;
+            mid = lo + (hi - lo) / 2;
         }
         if (lane == 0) ts.cut = lo;
     }
     group_sync<NW>();
     const uint32_t cut = ts.cut;
     const float cutv = key_value(cut);
-    if (m >= cutv) {
-        const int at = atomicAdd(&ts.threads, 1);
-        ts.who[at] = (uint8_t)tid;
-    }
-    group_sync<NW>();
-    const int threads = ts.threads;
-    for (int i = wave; i < threads; i += NW) {
-        const int t = ts.who[i];
-        for (int64_t j = lane; j * NT + t < nvec; j += WAVE) {
-            const int at = (int)(j * NT + t);
-            float f[V];
-            Piece<T>::unpack(Piece<T>::load(x + (int64_t)at * V), f);
+    const int pieces = (nvec + NT - 1) / NT;
+    auto candidates = [&](int at) {
+        float f[V];
+        Piece<T>::unpack(Piece<T>::load(x + (int64_t)at * V), f);
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (f[e] >= cutv) push(ts, f[e], id0 + at * V + e);
+        for (int e = 0; e < V; ++e)
+            if (f[e] >= cutv) push(ts, f[e], id0 + at * V + e);
+    };
+    if (m >= cutv) {
+        if (pk.m2 < cutv) {
+            if (pk.at >= 0)
+                for (int u = 0; u < U; ++u)
+                    if (pk.at + u * NT < nvec) candidates(pk.at + u * NT);
+        } else if (pieces <= 2 * U) {
+            for (int at = tid; at < nvec; at += NT) candidates(at);
+        } else {
+            ts.who[atomicAdd(&ts.threads, 1)] = (uint8_t)tid;
         }
-        if (lane == 0 && t < rem) {
-            const float v = to_f32(x[nvec * V + t]);
-            if (v >= cutv) push(ts, v, id0 + nvec * V + t);
-        }
+    }
+    if (pieces > 2 * U) {                // a wave reads what such a thread owns
+        group_sync<NW>();
+        const int threads = ts.threads;
+        for (int w = wave; w < threads; w += NW)
+            for (int j = lane; j < pieces; j += WAVE) {
+                const int at = j * NT + ts.who[w];
+                if (at < nvec) candidates(at);
+            }
+    }
+    if (tid < rem) {
+        const float v = to_f32(x[nvec * V + tid]);
+        if (v >= cutv) push(ts, v, id0 + nvec * V + tid);
     }
     group_sync<NW>();
     int got = ts.n;
@@ -303,9 +356,11 @@ __device__ int best_scores(const T* x, int n, uint32_t id0, float m, int top, in
     return got;
 }
 
-// what a row says, from its sums: log p of the ids, the entropy; or the distillation loss
+// What a row says, from its sums: log p of the ids, the entropy; or the distillation loss.  id, teacher, given: the thread's first
+// slot (NT or, for the loss, 64 slots are held by the threads), the teacher's score of it and the row's
 template <typename T, int NT, bool DISTILL>
-__device__ __forceinline__ void row_answer(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, int tid) {
+__device__ __forceinline__ void row_answer(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, int tid, int64_t id,
+                                           float teacher, float given) {
     const bool some = !(s.S == 0.f);
     const float l2 = some ? log2f(s.S) : INFINITY;
     if constexpr (!DISTILL) {
@@ -317,38 +372,54 @@ __device__ __forceinline__ void row_answer(const ScoreArgs& a, int64_t r, const 
             }
         }
         for (int k = tid; k < a.n_ids; k += NT) {
-            const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+            if (k != tid) {
+                id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                if (id >= 0 && id < a.c) given = to_f32(x[id]);
+            }
             float v = 0.f;
             if (id >= a.c) {
                 v = NAN;
                 if (a.id_status) flag_bad_id(a.id_status);
             } else if (id >= 0) {
-                v = some ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : -INFINITY;
+                v = some ? (given - s.m) * a.rt - LN2 * l2 : -INFINITY;
             }
             a.logp[r * a.n_ids + k] = v;
         }
     } else if (tid < WAVE) {                          // the list is short: one wave reads it three times
+        const int64_t id0 = id;
+        const float t0 = teacher, x0 = given;
+        auto slot = [&](int k) {
+            if (k == tid) {
+                id = id0;
+                teacher = t0;
+                given = x0;
+            } else {
+                id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                teacher = load_any(a.teacher, a.t_type, r * a.n_ids + k);
+                given = id >= 0 && id < a.c ? to_f32(x[id]) : 0.f;
+            }
+        };
         float mt = -FLT_MAX;
         for (int k = tid; k < a.n_ids; k += WAVE) {
-            const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
-            if (id >= 0) mt = fmaxf(mt, load_any(a.teacher, a.t_type, r * a.n_ids + k));
+            slot(k);
+            if (id >= 0) mt = fmaxf(mt, teacher);
             if (id >= a.c && a.id_status) flag_bad_id(a.id_status);
         }
         mt = wave_max(mt);
         float st = 0.f;
         for (int k = tid; k < a.n_ids; k += WAVE) {
-            const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
-            if (id >= 0) st += exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2);
+            slot(k);
+            if (id >= 0) st += exp2_raw((teacher - mt) * a.c2);
         }
         st = wave_sum(st);
         const float lt = st == 0.f ? INFINITY : log2f(st);
         float loss = 0.f;
         for (int k = tid; k < a.n_ids; k += WAVE) {
-            const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+            slot(k);
             if (id < 0) continue;
-            const float zt = load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt;
+            const float zt = teacher - mt;
             const float q = exp2_raw(zt * a.c2 - lt);
-            const float lp = id < a.c ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : NAN;
+            const float lp = id < a.c ? (given - s.m) * a.rt - LN2 * l2 : NAN;
             if (!(q == 0.f)) loss = fmaf(q, (zt * a.rt - LN2 * lt) - lp, loss);
         }
         loss = wave_sum(loss) * (a.t * a.t);
@@ -364,23 +435,31 @@ __device__ __forceinline__ void row_answer(const ScoreArgs& a, int64_t r, const 
     }
 }
 
-// orders `got` unordered keys and writes the best `top`: as a row's alternatives, or (keys != null) as keys
-template <typename T, int NT>
-__device__ __forceinline__ void write_best(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, const uint64_t* buf, int got,
+// Orders `got` unordered keys and writes the best `top`: as a row's alternatives, or (keys != null) as keys.  buf has room for
+// `got` rounded up to whole eights.
+template <typename T, int NW>
+__device__ __forceinline__ void write_best(const ScoreArgs& a, int64_t r, const T* x, const Sums& s, uint64_t* buf, int got,
                                            uint64_t* keys, int tid) {
+    constexpr int NT = NW * WAVE;
     const float ll = LN2 * log2f(s.S);
     const bool nan = s.S != s.S;
+    const int g8 = (got + 7) & ~7;
+    if (tid < g8 - got) buf[got + tid] = 0;
+    group_sync<NW>();
     for (int i = tid; i < got; i += NT) {
         const uint64_t mine = buf[i];
         int rank = 0;
-        for (int j = 0; j < got; ++j) rank += buf[j] > mine ? 1 : 0;
+        for (int j = 0; j < g8; j += 8)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rank += buf[j + e] > mine ? 1 : 0;
         if (rank >= a.top) continue;
         if (keys) {
-            keys[rank] = mine;
+            keys[rank] = mine >> 32 ? mine : 0;
         } else {
             const uint32_t id = ~(uint32_t)mine;
-            a.top_ids[r * a.top + rank] = nan ? -1 : (int64_t)id;
-            a.top_logp[r * a.top + rank] = nan ? NAN : (to_f32(x[id]) - s.m) * a.rt - ll;
+            const bool some = !nan && mine >> 32;
+            a.top_ids[r * a.top + rank] = some ? (int64_t)id : -1;
+            a.top_logp[r * a.top + rank] = nan ? NAN : some ? (to_f32(x[id]) - s.m) * a.rt - ll : -INFINITY;
         }
     }
     for (int i = got + tid; i < a.top; i += NT) {
@@ -393,64 +472,80 @@ __device__ __forceinline__ void write_best(const ScoreArgs& a, int64_t r, const 
     }
 }
 
-// NW waves a slice of a row; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best keys
+// blocks of 256 threads that a unit holds at once
+constexpr int score_fwd_blocks(bool top) { return top ? 6 : 8; }
+
+// NW waves a slice of a row; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best keys.
 template <typename T, int NW, bool ENT, bool TOP, bool DISTILL>
-__global__ void __launch_bounds__(SC_TPB) score_fwd_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(SC_TPB, score_fwd_blocks(TOP)) score_fwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
     __shared__ float scratch[GROUPS][3 * NW];
     __shared__ TopScratch<NW> top_scratch[TOP ? GROUPS : 1];
-    const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1);
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x & (NT - 1);
     const int64_t units = a.rows * a.splits;
     for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
         const int64_t r = a.splits == 1 ? unit : unit / a.splits;
-        const int64_t from = (unit - r * a.splits) * a.per;
+        const int from = (int)((unit - r * a.splits) * a.per);
+        const int n = (int)(a.per < a.c - from ? a.per : a.c - from);
+        const int nvec = n / V, rem = n - nvec * V;
         const T* row = row_ptr<T>(a.x, r);
         const T* x = row + from;
-        const int n = (int)(from + a.per < a.c ? a.per : a.c - from);
-        const int nvec = n / V, rem = n - nvec * V;
+        // the first id of this thread, and further down what the row says about it: both are back before they are needed
+        int64_t id = -1;
+        float teacher = 0.f, given = 0.f;
+        if (a.splits == 1 && tid < a.n_ids && (!DISTILL || tid < WAVE)) {
+            id = load_id(a.ids, a.id_type, r * a.n_ids + tid);
+            if constexpr (DISTILL) teacher = load_any(a.teacher, a.t_type, r * a.n_ids + tid);
+        }
         Sums s{-FLT_MAX, 0.f, 0.f};
-        int64_t j = tid;
-        const T* p = x + (int64_t)tid * V;
-        for (; j - tid + U * NT <= nvec; j += U * NT, p += (int64_t)U * NT * V) {
+        Peak pk{-FLT_MAX, -FLT_MAX, -1};
+        int j = 0;
+        const T* p = x + tid * V;
+        for (; j + U * NT <= nvec; j += U * NT, p += U * NT * V) {
             u32x4 raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = Piece<T>::load(p + (int64_t)u * NT * V);
+            for (int u = 0; u < U; ++u) raw[u] = Piece<T>::load(p + u * NT * V);
             float v[U * V];
 #pragma unroll
             for (int u = 0; u < U; ++u) Piece<T>::unpack(raw[u], *(float(*)[V])(v + u * V));
-            add_scores<ENT>(s, v, a.c2);
+            const float mx = add_scores<ENT>(s, v, a.c2);
+            if constexpr (TOP) pk.add(mx, j + tid);
         }
-        if (j - tid < nvec) {                         // the last pieces: past the end the last one again, masked
+        if (id >= 0 && id < a.c) given = to_f32(row[id]);
+        if (j < nvec) {                               // the last pieces: past the end the last one again, masked
             u32x4 raw[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t at = j + u * NT;
-                raw[u] = Piece<T>::load(x + (at < nvec ? at : nvec - 1) * V);
+                const int at = j + tid + u * NT;
+                if (j + u * NT < nvec) raw[u] = Piece<T>::load(x + (int64_t)(at < nvec ? at : nvec - 1) * V);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float v[V];
-                Piece<T>::unpack(raw[u], v);
-                const bool in = j + u * NT < nvec;
+                if (j + u * NT < nvec) {
+                    float v[V];
+                    Piece<T>::unpack(raw[u], v);
+                    const bool in = j + tid + u * NT < nvec;
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = in ? v[e] : -INFINITY;
-                if (j - tid + u * NT < nvec) add_scores<ENT>(s, v, a.c2);
+                    for (int e = 0; e < V; ++e) v[e] = in ? v[e] : -INFINITY;
+                    const float mx = add_scores<ENT>(s, v, a.c2);
+                    if constexpr (TOP) pk.add(mx, j + tid);
+                }
             }
         }
         if (rem) {
             const float v[1] = {tid < rem ? to_f32(x[nvec * V + tid]) : -INFINITY};
-            add_scores<ENT>(s, v, a.c2);
+            const float mx = add_scores<ENT>(s, v, a.c2);
+            if constexpr (TOP) pk.add(mx, -1);
         }
-        const float m = s.m;
         s = group_sums<NW, ENT>(s, a.c2, scratch[group]);
         if (a.splits == 1) {
-            row_answer<T, NT, DISTILL>(a, r, row, s, tid);
+            row_answer<T, NT, DISTILL>(a, r, row, s, tid, id, teacher, given);
         } else if (tid == 0) {
             a.part[unit] = make_float4(s.m, s.S, s.W, 0.f);
         }
         if constexpr (TOP) {
-            const int got = best_scores<T, NW>(x, n, (uint32_t)from, m, a.top, tid, top_scratch[group]);
-            write_best<T, NT>(a, r, row, s, top_scratch[group].key, got, a.splits == 1 ? nullptr : a.keys + unit * a.top, tid);
+            const int got = best_scores<T, NW>(x, n, (uint32_t)from, pk, a.top, tid, top_scratch[group]);
+            write_best<T, NW>(a, r, row, s, top_scratch[group].key, got, a.splits == 1 ? nullptr : a.keys + unit * a.top, tid);
         }
         group_sync<NW>();                             // the scratch is free again
     }
@@ -460,67 +555,119 @@ __global__ void __launch_bounds__(SC_TPB) score_fwd_kernel(ScoreArgs a) {
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
     __shared__ float scratch[3 * SC_NW];
-    __shared__ uint64_t buf[TOP ? SC_MAX_TOP * SC_MAX_TOP : 1];
-    __shared__ uint64_t heads[TOP ? SC_TPB : 1];
+    __shared__ uint64_t scratch64[SC_NW];
+    __shared__ uint64_t buf[TOP ? SC_MAX_TOP * SC_MAX_TOP + 8 : 1];
+    __shared__ uint64_t heads[TOP ? SC_TPB + 8 : 1];
     __shared__ uint64_t cut;
-    __shared__ int got;
+    __shared__ int n, lists;
+    __shared__ uint8_t who[SC_TPB];
     const int tid = threadIdx.x;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = row_ptr<T>(a.x, r);
+        int64_t id = -1;
+        float teacher = 0.f, given = 0.f;
+        if (tid < a.n_ids && (!DISTILL || tid < WAVE)) {
+            id = load_id(a.ids, a.id_type, r * a.n_ids + tid);
+            if constexpr (DISTILL) teacher = load_any(a.teacher, a.t_type, r * a.n_ids + tid);
+        }
+        // Every slice's q-th best key, q = top / slices rounded up: the m-th largest of them, m q >= top, bounds the row's best
+        const int q = TOP ? (a.top + a.splits - 1) / a.splits : 1, m = TOP ? (a.top + q - 1) / q : 1;
+        uint64_t head = 0;
         Sums s{-FLT_MAX, 0.f, 0.f};
         if (tid < a.splits) {
             const float4 p = a.part[r * a.splits + tid];
             s = Sums{p.x, p.y, p.z};
+            if constexpr (TOP) head = a.keys[(r * a.splits + tid) * a.top + q - 1];
         }
-        s = group_sums<SC_NW, ENT>(s, a.c2, scratch);
-        row_answer<T, SC_TPB, DISTILL>(a, r, x, s, tid);
+        if (id >= 0 && id < a.c) given = to_f32(x[id]);
         if constexpr (TOP) {
-            const uint64_t* keys = a.keys + (r * a.splits + tid) * a.top;
-            const uint64_t head = tid < a.splits ? keys[0] : 0;
             heads[tid] = head;
+            if (tid < 8) heads[SC_TPB + tid] = 0;
             if (tid == 0) {
                 cut = 1;
-                got = 0;
+                n = lists = 0;
             }
-            __syncthreads();
-            if (head) {                               // the top-th best of the slices' best keys is a bound for all
-                int rank = 0;
-                for (int i = 0; i < a.splits; ++i) rank += heads[i] > head ? 1 : 0;
-                if (rank == a.top - 1) cut = head;
-            }
-            __syncthreads();
+        }
+        s = group_sums<SC_NW, ENT>(s, a.c2, scratch);             // (its barrier is the one that `heads` needs)
+        row_answer<T, SC_TPB, DISTILL>(a, r, x, s, tid, id, teacher, given);
+        if constexpr (TOP) {
             if (head) {
-                for (int i = 0; i < a.top; ++i) {
-                    const uint64_t k = keys[i];
-                    if (k < cut) break;
-                    buf[atomicAdd(&got, 1)] = k;
-                }
+                int rank = 0;
+                for (int i = 0; i < a.splits; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) rank += heads[i + e] > head ? 1 : 0;
+                if (rank == m - 1) cut = head;
             }
             __syncthreads();
-            write_best<T, SC_TPB>(a, r, x, s, buf, got, nullptr, tid);
+            // the slices that can have keys that good: with q = 1 those whose best is, else (fewer than top) all
+            if (tid < a.splits && (q > 1 || head >= cut)) who[atomicAdd(&lists, 1)] = (uint8_t)tid;
+            __syncthreads();
+            const uint64_t* all = a.keys + r * a.splits * a.top;
+            const int items = lists * a.top;
+            for (int i0 = tid; i0 < items; i0 += 4 * SC_TPB) {
+                uint64_t k[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * SC_TPB, w = i / a.top;
+                    k[u] = i < items ? all[who[w] * a.top + i - w * a.top] : 0;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (k[u] >= cut) buf[atomicAdd(&n, 1)] = k[u];
+            }
+            __syncthreads();
+            int got = n;
+            if (got > SC_BUF) {                       // ties in many slices: one after the other, into the place of the heads
+                uint64_t last = ~(uint64_t)0;
+                for (int k = 0; k < a.top; ++k) {
+                    uint64_t best = 0;
+                    for (int i = tid; i < got; i += SC_TPB)
+                        if (buf[i] < last && buf[i] > best) best = buf[i];
+                    last = block_max_u64<SC_NW>(best, scratch64);
+                    if (tid == 0) heads[k] = last;
+                }
+                __syncthreads();
+                write_best<T, SC_NW>(a, r, x, s, heads, a.top, nullptr, tid);
+            } else {
+                write_best<T, SC_NW>(a, r, x, s, buf, got, nullptr, tid);
+            }
         }
         __syncthreads();
     }
 }
 
-// Slices of a row.  Rows alone fill the chip (8 blocks of 256 threads on each of 256 units) from 2048 on; fewer are cut into
-// slices of at least 4096 scores, at most one for each thread of the kernel that joins them.
-static int score_splits(int64_t rows, int64_t c) {
-    if (rows >= 2048 || c < 8192) return 1;
-    int64_t n = (2048 + rows - 1) / (rows < 1 ? 1 : rows);
-    if (n > c / 4096) n = c / 4096;
-    if (n > SC_TPB) n = SC_TPB;
-    return (int)(n < 1 ? 1 : n);
+// Slices of a row: what makes rounds(slices) * (a slice's length + what a slice costs beside reading it) + the joining kernel
+// smallest.  The costs are in scores that a block of a full chip reads meanwhile (2.7 KB/us of 16-bit scores): about 2 us a slice,
+// 5 us with alternatives, 5 us for the second kernel.  No slice is below 4096 scores; the joining kernel has a thread for each.
+static int score_splits(int64_t rows, int64_t c, int top) {
+    if (c < 8192) return 1;
+    const int64_t slots = (int64_t)device_cu_count() * score_fwd_blocks(top > 0), own = top ? 6700 : 2700;
+    int64_t most = c / 4096 < SC_TPB ? c / 4096 : SC_TPB, best = 0;
+    int n = 1;
+    for (int64_t k = 1; k <= most; ++k) {
+        const int64_t cost = (rows * k + slots - 1) / slots * (c / k + own) + (k > 1 ? 6700 : 0);
+        if (k == 1 || cost < best) {
+            best = cost;
+            n = (int)k;
+        }
+    }
+    return n;
+}
+
+// blocks that take slice after slice: at most what the chip holds at once
+static unsigned score_grid(int64_t blocks, int per_unit) {
+    const int64_t most = (int64_t)device_cu_count() * per_unit;
+    return (unsigned)(blocks < most ? blocks : most);
 }
 
 static int64_t score_ws(int64_t rows, int64_t c, int top) {
-    const int64_t splits = score_splits(rows, c);
+    const int64_t splits = score_splits(rows, c, top);
     return splits == 1 ? 0 : rows * splits * (16 + (int64_t)top * 8);
 }
 
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 static int launch_score_fwd(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
-    a.splits = score_splits(a.rows, a.c);
+    a.splits = score_splits(a.rows, a.c, a.top);
     a.per = a.splits == 1 ? a.c : ((a.c + a.splits - 1) / a.splits + 63) / 64 * 64;
     if (a.splits > 1) {
         if (!ws || ws_bytes < score_ws(a.rows, a.c, a.top)) return ARMNET_ERR_BAD_ARG;
@@ -528,11 +675,13 @@ static int launch_score_fwd(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_
         a.part = (float4*)ws;
         a.keys = (uint64_t*)(a.part + a.rows * a.splits);
     }
-    // a wave a row as long as its lanes hold the row in one go
-    if (a.c <= WAVE * Piece<T>::N * SC_UNROLL)
-        score_fwd_kernel<T, 1, ENT, TOP, DISTILL><<<row_grid((a.rows + 3) / 4), SC_TPB, 0, st>>>(a);
+    // A wave a row: what a row costs beside reading it is paid once instead of by four waves.  For short rows always, for longer ones
+    // where rows alone fill the chip (8191 x 5382 f16: 27.2 us with a block a row, 23.5 with a wave; 4096 rows: 12.8, 10.3)
+    const int64_t one_go = WAVE * Piece<T>::N * 4;
+    if (a.c <= one_go || (a.splits == 1 && a.rows >= 4096 && a.c <= 16 * one_go))
+        score_fwd_kernel<T, 1, ENT, TOP, DISTILL><<<score_grid((a.rows + 3) / 4, score_fwd_blocks(TOP)), SC_TPB, 0, st>>>(a);
     else
-        score_fwd_kernel<T, SC_NW, ENT, TOP, DISTILL><<<row_grid(a.rows * a.splits), SC_TPB, 0, st>>>(a);
+        score_fwd_kernel<T, SC_NW, ENT, TOP, DISTILL><<<score_grid(a.rows * a.splits, score_fwd_blocks(TOP)), SC_TPB, 0, st>>>(a);
     ARMNET_LAUNCH_CHECK();
     if (a.splits > 1) {
         score_join_kernel<T, ENT, TOP, DISTILL><<<row_grid(a.rows), SC_TPB, 0, st>>>(a);
@@ -554,7 +703,7 @@ template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
     extern __shared__ int4 lists[];
-    const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1), lane = tid & (WAVE - 1);
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x & (NT - 1), lane = tid & (WAVE - 1);
     const int n4 = (a.n_ids + 3) & ~3;
     int32_t* s_id = (int32_t*)lists + group * 2 * n4;
     float* s_g = (float*)(s_id + n4);
@@ -665,7 +814,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
 
 template <typename T, bool ENT, bool DISTILL>
 static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
-    const bool narrow = a.c <= WAVE * Piece<T>::N * SC_UNROLL;
+    const bool narrow = a.c <= WAVE * Piece<T>::N * 4;
     // slices of at most 65536 scores; few rows: down to what a block's threads load at once
     const int64_t at_once = SC_TPB * Piece<T>::N * SC_UNROLL;
     int64_t splits = (a.c + 65535) / 65536;
