@@ -51,47 +51,105 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v) {
     else ((f16_t*)p)[i] = (f16_t)v;
 }
 
-// a piece of which only the first `n` elements are there; the others read as 0 and are not written
-template <typename T>
-__device__ __forceinline__ u32x4 load_some(const T* p, int n) {
-    constexpr int V = Piece<T>::N;
-    if (n >= V) return Piece<T>::load(p);
-    float f[V];
+// The elements of a row that a lane holds: NV pieces of V.  Piece i is [at, at + V) with at = (i * NT + tid) * V; past the row's
+// end it is pulled back to the row's last V elements, so that every load is a whole one inside the row, and only the elements from
+// `lo` on are the lane's own (all: 0, none: V).  Rows shorter than V (one lane each) are read element by element.
+template <typename T, int NT, int NV>
+struct Columns {
+    static constexpr int V = Piece<T>::N;
+    int off[NV], lo[NV];
+    bool tiny;
+    int d;
+    __device__ __forceinline__ Columns(int d_, int tid) : d(d_) {
+        tiny = NT == 1 && d < V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = e < n ? to_f32(p[e]) : 0.f;
-    return Piece<T>::pack(f);
-}
-
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, int n, const float (&f)[Piece<T>::N]) {
-    constexpr int V = Piece<T>::N;
-    if (n >= V) {
-        Piece<T>::store(p, Piece<T>::pack(f));
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (e < n) p[e] = from_f32<T>(f[e]);
+        for (int i = 0; i < NV; ++i) {
+            const int at = (i * NT + tid) * V;
+            off[i] = at + V <= d ? at : (d < V ? 0 : d - V);
+            lo[i] = at - off[i] < V ? at - off[i] : V;
+        }
     }
-}
+    __device__ __forceinline__ void load(const T* row, u32x4 (&raw)[NV]) const {
+        if (NT == 1 && tiny) {
+            float f[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = e < d ? to_f32(row[e]) : 0.f;
+            raw[0] = Piece<T>::pack(f);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = Piece<T>::load(row + off[i]);
+    }
+    // what is not the lane's own counts as 0 in sums
+    __device__ __forceinline__ void own(int i, float (&f)[V]) const {
+        if (NT == 1) {
+            if (tiny)
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] = e < d ? f[e] : 0.f;
+        } else if (lo[i]) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = e >= lo[i] ? f[e] : 0.f;
+        }
+    }
+    __device__ __forceinline__ bool has(int i, int e) const { return NT == 1 ? !tiny || e < d : e >= lo[i]; }
+    __device__ __forceinline__ void store(T* row, int i, const float (&f)[V]) const {
+        if (NT == 1 ? !tiny : lo[i] == 0) {
+            Piece<T>::store(row + off[i], Piece<T>::pack(f));
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (has(i, e)) row[off[i] + e] = from_f32<T>(f[e]);
+        }
+    }
+    // a parameter's values, `fill` without one
+    template <typename W>
+    __device__ __forceinline__ void param_of(const W* p, float (&f)[NV][V]) const {
+        if (NT == 1 && tiny) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[0][e] = e < d ? to_f32(p[e]) : 0.f;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; e += Piece<W>::N) {
+                if constexpr (Piece<W>::N <= V) {
+                    Piece<W>::unpack(Piece<W>::load(p + off[i] + e), *(float(*)[Piece<W>::N])(f[i] + e));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) f[i][k] = to_f32(p[off[i] + k]);
+                }
+            }
+    }
+    __device__ __forceinline__ void param(const void* p, int type, float fill, float (&f)[NV][V]) const {
+        if (!p) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[i][e] = fill;
+        } else if (type == ARMNET_F32) {
+            param_of((const float*)p, f);
+        } else if (type == ARMNET_BF16) {
+            param_of((const bf16_t*)p, f);
+        } else {
+            param_of((const f16_t*)p, f);
+        }
+    }
+};
 
 // sum over the lanes (and waves) that hold a row, in each of them; scratch: one float a wave, of this sum alone
 template <int LPR, int NW>
 __device__ __forceinline__ float row_sum(float v, float* scratch) {
-    if constexpr (LPR < WAVE) {
+    if constexpr (LPR < WAVE) return lanes_sum<LPR>(v);
+    v = wave_sum(v);
+    if constexpr (NW == 1) return v;
+    const int wave = threadIdx.x / WAVE;
+    if ((threadIdx.x & (WAVE - 1)) == 0) scratch[wave] = v;
+    __syncthreads();
+    v = 0.f;
 #pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) v += __shfl_xor(v, d);
-        return v;
-    } else {
-        v = wave_sum(v);
-        if constexpr (NW == 1) return v;
-        const int wave = threadIdx.x / WAVE;
-        if ((threadIdx.x & (WAVE - 1)) == 0) scratch[wave] = v;
-        __syncthreads();
-        v = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) v += scratch[wave / NW * NW + i];
-        return v;
-    }
+    for (int i = 0; i < NW; ++i) v += scratch[wave / NW * NW + i];
+    return v;
 }
 
 // One row group: LPR lanes (NW = 1) or NW waves.  A block holds TPB / (LPR or NW * 64) of them.
@@ -100,65 +158,50 @@ __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
     constexpr int V = Piece<T>::N, NT = LPR < WAVE ? LPR : NW * WAVE, GROUPS = TPB / NT;
     __shared__ float scratch[2][TPB / WAVE];
     const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1);
-    float w[NV][V], b[NV][V];
-    int cnt[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + tid) * V;
-        cnt[i] = a.d - at < 0 ? 0 : a.d - at < V ? a.d - at : V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            w[i][e] = a.weight && e < cnt[i] ? load_param(a.weight, a.w_type, at + e) : 1.f;
-            b[i][e] = a.bias && e < cnt[i] ? load_param(a.bias, a.w_type, at + e) : 0.f;
-        }
-    }
-    const float rd = 1.f / (float)a.d;
+    const Columns<T, NT, NV> cols(a.d, tid);
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     const int64_t rounds = (a.rows + step - 1) / step;
-    auto load = [&](int64_t r, u32x4 (&raw)[NV]) {
-        const T* x = row_ptr<T>(a.x, r < a.rows ? r : a.rows - 1);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (cnt[i]) raw[i] = load_some(x + (i * NT + tid) * V, cnt[i]);
-    };
-    u32x4 raw[NV] = {}, next[NV] = {};
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    load(r, raw);
+    u32x4 raw[NV];
+    cols.load(row_ptr<T>(a.x, r < a.rows ? r : a.rows - 1), raw);
+    float w[NV][V], b[NV][V];
+    cols.param(a.weight, a.w_type, 1.f, w);
+    cols.param(a.bias, a.w_type, 0.f, b);
     for (int64_t k = 0; k < rounds; ++k, r += step) {
-        if (k + 1 < rounds) load(r + step, next);
         float f[NV][V];
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             Piece<T>::unpack(raw[i], f[i]);
+            cols.own(i, f[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) s += f[i][e];
         }
+        if (k + 1 < rounds) cols.load(row_ptr<T>(a.x, r + step < a.rows ? r + step : a.rows - 1), raw);
         const float mean = row_sum<LPR, NW>(s, scratch[0]) / (float)a.d;     // a constant row is its own mean
         float q = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                f[i][e] = e < cnt[i] ? f[i][e] - mean : 0.f;
-                q = fmaf(f[i][e], f[i][e], q);
-            }
-        const float rstd = 1.f / sqrtf(row_sum<LPR, NW>(q, scratch[1]) * rd + a.eps);
+            for (int e = 0; e < V; ++e) f[i][e] -= mean;
+            cols.own(i, f[i]);
+#pragma unroll
+            for (int e = 0; e < V; ++e) q = fmaf(f[i][e], f[i][e], q);
+        }
+        const float rstd = 1.f / sqrtf(row_sum<LPR, NW>(q, scratch[1]) / (float)a.d + a.eps);
         if (r < a.rows) {
             T* y = (T*)a.out + r * a.d;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) f[i][e] = fmaf(f[i][e] * rstd, w[i][e], b[i][e]);
-                if (cnt[i]) store_some(y + (i * NT + tid) * V, cnt[i], f[i]);
+                cols.store(y, i, f[i]);
             }
             if (tid == 0 && a.mean) {
                 a.mean[r] = mean;
                 a.rstd[r] = rstd;
             }
         }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = next[i];
     }
 }
 
@@ -166,55 +209,45 @@ __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
 template <typename T, int LPR, int NW, int NV, int TPB>
 __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
     constexpr int V = Piece<T>::N, NT = LPR < WAVE ? LPR : NW * WAVE, GROUPS = TPB / NT;
-    __shared__ float scratch[2][TPB / WAVE];
+    __shared__ float scratch[2][2][TPB / WAVE];
     constexpr int SHARES = LPR < WAVE ? TPB / WAVE : GROUPS;     // short rows: a wave's groups meet in registers
     __shared__ float sums[2][SHARES > 1 ? NV * NT * V : 1];
     const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1);
-    float w[NV][V], dw[NV][V] = {}, db[NV][V] = {};
-    int cnt[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + tid) * V;
-        cnt[i] = a.d - at < 0 ? 0 : a.d - at < V ? a.d - at : V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[i][e] = a.weight && e < cnt[i] ? load_param(a.weight, a.w_type, at + e) : 1.f;
-    }
+    const Columns<T, NT, NV> cols(a.d, tid);
     const float rd = 1.f / (float)a.d;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     const int64_t rounds = (a.rows + step - 1) / step;
-    struct Row {
-        u32x4 x[NV], dy[NV];
-        float mean, rstd;
+    u32x4 rx[NV], ry[NV];
+    float mean, rstd;
+    auto load = [&](int64_t r) {                       // a group without a row works on the last one's values and drops them
+        const int64_t q = r < a.rows ? r : a.rows - 1;
+        cols.load(row_ptr<T>(a.x, q), rx);
+        cols.load((const T*)a.dy + q * a.d, ry);
+        mean = a.mean[q];
+        rstd = a.rstd[q];
     };
-    auto load = [&](int64_t r, Row& o) {
-        const bool in = r < a.rows;                    // a group without a row works on the last one's values and drops them
-        const int64_t q = in ? r : a.rows - 1;
-        const T* x = row_ptr<T>(a.x, q);
-        const T* dy = (const T*)a.dy + q * a.d;
-        o.mean = a.mean[q];
-        o.rstd = a.rstd[q];
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (cnt[i]) {
-                o.x[i] = load_some(x + (i * NT + tid) * V, cnt[i]);
-                o.dy[i] = load_some(dy + (i * NT + tid) * V, cnt[i]);
-            }
-    };
-    Row cur = {}, next = {};
     int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-    load(r, cur);
+    load(r);
+    float w[NV][V], dw[NV][V] = {}, db[NV][V] = {};
+    cols.param(a.weight, a.w_type, 1.f, w);
     for (int64_t k = 0; k < rounds; ++k, r += step) {
-        if (k + 1 < rounds) load(r + step, next);
         const bool in = r < a.rows;
+        const float rs = rstd;
         float h[NV][V], g[NV][V];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            Piece<T>::unpack(cur.x[i], h[i]);
-            Piece<T>::unpack(cur.dy[i], g[i]);
+            Piece<T>::unpack(rx[i], h[i]);
+            Piece<T>::unpack(ry[i], g[i]);
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[i][e] = (h[i][e] - mean) * rs;
+            cols.own(i, g[i]);                         // 0 in g makes 0 of everything below
+        }
+        if (k + 1 < rounds) load(r + step);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                h[i][e] = e < cnt[i] ? (h[i][e] - cur.mean) * cur.rstd : 0.f;
                 if (in) {
                     dw[i][e] = fmaf(g[i][e], h[i][e], dw[i][e]);
                     db[i][e] += g[i][e];
@@ -223,21 +256,40 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
                 s1 += g[i][e];
                 s2 = fmaf(g[i][e], h[i][e], s2);
             }
-        }
         if (a.out) {
-            const float m1 = row_sum<LPR, NW>(s1, scratch[0]) * rd;
-            const float m2 = row_sum<LPR, NW>(s2, scratch[1]) * rd;
+            float m1, m2;
+            if constexpr (NW == 1) {
+                m1 = row_sum<LPR, NW>(s1, nullptr) * rd;
+                m2 = row_sum<LPR, NW>(s2, nullptr) * rd;
+            } else {                                   // both through one barrier; the next row takes the other scratch
+                float(*sc)[TPB / WAVE] = scratch[k & 1];
+                const int wave = threadIdx.x / WAVE;
+                s1 = wave_sum(s1);
+                s2 = wave_sum(s2);
+                if ((threadIdx.x & (WAVE - 1)) == 0) {
+                    sc[0][wave] = s1;
+                    sc[1][wave] = s2;
+                }
+                __syncthreads();
+                m1 = m2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    m1 += sc[0][wave / NW * NW + i];
+                    m2 += sc[1][wave / NW * NW + i];
+                }
+                m1 *= rd;
+                m2 *= rd;
+            }
             if (in) {
                 T* dx = (T*)a.out + r * a.d;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) g[i][e] = cur.rstd * (g[i][e] - m1 - h[i][e] * m2);
-                    if (cnt[i]) store_some(dx + (i * NT + tid) * V, cnt[i], g[i]);
+                    for (int e = 0; e < V; ++e) g[i][e] = rs * (g[i][e] - m1 - h[i][e] * m2);
+                    cols.store(dx, i, g[i]);
                 }
             }
         }
-        cur = next;
     }
     if (!a.params) return;
     int share = group;
@@ -277,8 +329,8 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int col = (i * NT + tid) * V + e;
-                if (e >= cnt[i]) continue;
+                const int col = cols.off[i] + e;
+                if (!cols.has(i, e)) continue;
                 if (a.blocks == 1) {
                     if (a.dweight) store_param(a.dweight, a.w_type, col, dw[i][e]);
                     if (a.dbias) store_param(a.dbias, a.w_type, col, db[i][e]);
@@ -386,60 +438,95 @@ __global__ void __launch_bounds__(LN_TPB) norm_long_param_kernel(NormArgs a) {
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
 
-constexpr int LN_BWD_TPB = 1024;
+// Who holds a row of `np` 16-byte pieces: lpr lanes of a wave or nw waves, nv pieces a lane; tpb threads a block.
+struct NormShape {
+    int lpr, nw, nv, tpb;
+};
 
-// how many rows a block of the backward works on at a time: the groups of 16 waves (see launch_norm)
-static int norm_bwd_groups(int64_t d, int64_t v) {
-    const int64_t np = (d + v - 1) / v;
+// Few pieces a lane keep everything in registers.  A barrier's cost grows with the waves that meet at it.
+static NormShape norm_fwd_shape(int64_t np) {
     if (np <= WAVE) {
         int lpr = 1;
         while (lpr < np) lpr *= 2;
-        return LN_BWD_TPB / lpr;
+        return {lpr, 1, 1, LN_TPB};
     }
-    if (np <= 2 * WAVE) return 16;
-    if (np <= 8 * WAVE) return 4;
-    return 1;
+    if (np <= 128) return {WAVE, 1, 2, LN_TPB};
+    if (np <= 256) return {WAVE, 4, 1, LN_TPB};
+    if (np <= 512) return {WAVE, 4, 2, LN_TPB};        // (16384 x 4096 bf16: 46 us; eight waves with one piece a lane 55)
+    if (np <= 1024) return {WAVE, 16, 1, 1024};
+    if (np <= 2048) return {WAVE, 16, 2, 1024};
+    return {WAVE, 16, 4, 1024};
 }
 
-// Blocks of the backward, one a unit: 16 waves with a row in work and one on its way each keep enough bytes in flight, and fewer
-// blocks mean fewer shares of the parameters' gradients to add up.  (The 16-bit types' groups: never fewer rows than blocks need.)
-static int norm_blocks(int64_t rows, int64_t d, int64_t v) {
+// The backward keeps five values of a column (w, h, g and two sums): one piece a lane, then more registers a lane in smaller blocks.
+static NormShape norm_bwd_shape(int64_t np, int v) {
+    if (np <= WAVE) {
+        int lpr = 1;
+        while (lpr < np) lpr *= 2;
+        return {lpr, 1, 1, 1024};
+    }
+    if (np <= 128) return v == 4 ? NormShape{WAVE, 1, 2, 1024} : NormShape{WAVE, 2, 1, 1024};
+    if (np <= 256) return {WAVE, 4, 1, 1024};
+    if (np <= 512) return {WAVE, 8, 1, 1024};
+    if (np <= 1024) return {WAVE, 16, 1, 1024};
+    if (np <= 2048) return v == 4 ? NormShape{WAVE, 16, 2, 1024} : NormShape{WAVE, 8, 4, 512};
+    return {WAVE, 8, 8, 512};
+}
+
+static int64_t norm_groups(const NormShape& s) { return s.tpb / (s.lpr < WAVE ? s.lpr : s.nw * WAVE); }
+
+// Blocks of the backward, one a unit: its waves with a row in work and one on its way each keep enough bytes in flight, and fewer
+// blocks mean fewer shares of the parameters' gradients to add up.
+static int norm_blocks(int64_t rows, int64_t d, int v) {
     if (d > LN_MAX_D) return (int)(rows < 256 ? rows : 256);
-    const int64_t groups = norm_bwd_groups(d, v);
+    const int64_t groups = norm_groups(norm_bwd_shape((d + v - 1) / v, v));
     const int64_t n = (rows + groups - 1) / groups;
     return (int)(n < 256 ? n : 256);
 }
 
-template <typename T, int LPR, int NW, int NV, bool BWD>
-static void launch_norm_one(const NormArgs& a, hipStream_t st) {
-    if constexpr (BWD) {
-        norm_bwd_kernel<T, LPR, NW, NV, LN_BWD_TPB><<<a.blocks, LN_BWD_TPB, 0, st>>>(a);
-    } else {
-        constexpr int TPB = NW == 16 ? 1024 : LN_TPB, GROUPS = TPB / (LPR < WAVE ? LPR : NW * WAVE);
-        int64_t blocks = (a.rows + GROUPS - 1) / GROUPS;
-        const int64_t most = (int64_t)device_cu_count() * (NW == 16 ? 2 : 8);
-        if (blocks > most) blocks = most;
-        norm_fwd_kernel<T, LPR, NW, NV, TPB><<<(unsigned)blocks, TPB, 0, st>>>(a);
-    }
+template <typename T, int LPR, int NW, int NV, int TPB>
+static bool try_norm_fwd(const NormShape& s, const NormArgs& a, hipStream_t st) {
+    if (s.lpr != LPR || s.nw != NW || s.nv != NV || s.tpb != TPB) return false;
+    const int64_t groups = norm_groups(s), most = (int64_t)device_cu_count() * (2048 / TPB);
+    int64_t blocks = (a.rows + groups - 1) / groups;
+    if (blocks > most) blocks = most;
+    norm_fwd_kernel<T, LPR, NW, NV, TPB><<<(unsigned)blocks, TPB, 0, st>>>(a);
+    return true;
 }
 
-// who holds a row: by its number of 16-byte pieces
-template <typename T, bool BWD>
-static void launch_norm(const NormArgs& a, hipStream_t st) {
-    const int np = (a.d + Piece<T>::N - 1) / Piece<T>::N;
-    if (np <= 1) launch_norm_one<T, 1, 1, 1, BWD>(a, st);
-    else if (np <= 2) launch_norm_one<T, 2, 1, 1, BWD>(a, st);
-    else if (np <= 4) launch_norm_one<T, 4, 1, 1, BWD>(a, st);
-    else if (np <= 8) launch_norm_one<T, 8, 1, 1, BWD>(a, st);
-    else if (np <= 16) launch_norm_one<T, 16, 1, 1, BWD>(a, st);
-    else if (np <= 32) launch_norm_one<T, 32, 1, 1, BWD>(a, st);
-    else if (np <= 64) launch_norm_one<T, 64, 1, 1, BWD>(a, st);
-    else if (np <= 128) launch_norm_one<T, 64, 1, 2, BWD>(a, st);
-    else if (np <= 256) launch_norm_one<T, 64, 4, 1, BWD>(a, st);
-    else if (np <= 512) launch_norm_one<T, 64, 4, 2, BWD>(a, st);
-    else if (np <= 1024) launch_norm_one<T, 64, 16, 1, BWD>(a, st);
-    else if (np <= 2048) launch_norm_one<T, 64, 16, 2, BWD>(a, st);
-    else if constexpr (sizeof(T) == 4) launch_norm_one<T, 64, 16, 4, BWD>(a, st);
+template <typename T, int LPR, int NW, int NV, int TPB>
+static bool try_norm_bwd(const NormShape& s, const NormArgs& a, hipStream_t st) {
+    if (s.lpr != LPR || s.nw != NW || s.nv != NV || s.tpb != TPB) return false;
+    norm_bwd_kernel<T, LPR, NW, NV, TPB><<<a.blocks, TPB, 0, st>>>(a);
+    return true;
+}
+
+template <typename T>
+static bool launch_norm_fwd(const NormArgs& a, hipStream_t st) {
+    const NormShape s = norm_fwd_shape((a.d + Piece<T>::N - 1) / Piece<T>::N);
+    if (try_norm_fwd<T, 1, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 2, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 4, 1, 1, 256>(s, a, st) ||
+        try_norm_fwd<T, 8, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 16, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 32, 1, 1, 256>(s, a, st) ||
+        try_norm_fwd<T, 64, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 64, 1, 2, 256>(s, a, st) || try_norm_fwd<T, 64, 4, 1, 256>(s, a, st) ||
+        try_norm_fwd<T, 64, 4, 2, 256>(s, a, st) || try_norm_fwd<T, 64, 16, 1, 1024>(s, a, st) ||
+        try_norm_fwd<T, 64, 16, 2, 1024>(s, a, st))
+        return true;
+    if constexpr (sizeof(T) == 4) return try_norm_fwd<T, 64, 16, 4, 1024>(s, a, st);
+    return false;
+}
+
+template <typename T>
+static bool launch_norm_bwd(const NormArgs& a, hipStream_t st) {
+    constexpr int V = Piece<T>::N;
+    const NormShape s = norm_bwd_shape((a.d + V - 1) / V, V);
+    if (try_norm_bwd<T, 1, 1, 1, 1024>(s, a, st) || try_norm_bwd<T, 2, 1, 1, 1024>(s, a, st) || try_norm_bwd<T, 4, 1, 1, 1024>(s, a, st) ||
+        try_norm_bwd<T, 8, 1, 1, 1024>(s, a, st) || try_norm_bwd<T, 16, 1, 1, 1024>(s, a, st) || try_norm_bwd<T, 32, 1, 1, 1024>(s, a, st) ||
+        try_norm_bwd<T, 64, 1, 1, 1024>(s, a, st) || try_norm_bwd<T, 64, 4, 1, 1024>(s, a, st) || try_norm_bwd<T, 64, 8, 1, 1024>(s, a, st) ||
+        try_norm_bwd<T, 64, 16, 1, 1024>(s, a, st))
+        return true;
+    if constexpr (sizeof(T) == 4)
+        return try_norm_bwd<T, 64, 1, 2, 1024>(s, a, st) || try_norm_bwd<T, 64, 16, 2, 1024>(s, a, st) || try_norm_bwd<T, 64, 8, 8, 512>(s, a, st);
+    else
+        return try_norm_bwd<T, 64, 2, 1, 1024>(s, a, st) || try_norm_bwd<T, 64, 8, 4, 512>(s, a, st);
 }
 
 }  // namespace armnet
@@ -462,7 +549,9 @@ int armnet_layer_norm_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int
     a.w_type = w_type; a.weight = weight; a.bias = bias; a.eps = eps; a.out = y; a.mean = mean; a.rstd = rstd;
     hipStream_t st = (hipStream_t)stream;
     if (d <= LN_MAX_D) {
-        ARMNET_ROW_TYPE(x_type, T, (launch_norm<T, false>(a, st)));
+        bool there = false;
+        ARMNET_ROW_TYPE(x_type, T, there = launch_norm_fwd<T>(a, st));
+        if (!there) return ARMNET_ERR_UNSUPPORTED;
     } else {
         ARMNET_ROW_TYPE(x_type, T, (norm_long_fwd_kernel<T><<<row_grid(rows), LN_TPB, 0, st>>>(a)));
     }
@@ -495,7 +584,9 @@ int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int
     a.blocks = norm_blocks(rows, d, x_type == ARMNET_F32 ? 4 : 8);
     if (rows > 0 && (dx || params)) {
         if (d <= LN_MAX_D) {
-            ARMNET_ROW_TYPE(x_type, T, (launch_norm<T, true>(a, st)));
+            bool there = false;
+            ARMNET_ROW_TYPE(x_type, T, there = launch_norm_bwd<T>(a, st));
+            if (!there) return ARMNET_ERR_UNSUPPORTED;
             ARMNET_LAUNCH_CHECK();
             if (a.blocks == 1) return ARMNET_OK;                     // the one block has written the parameters' gradients
         } else {

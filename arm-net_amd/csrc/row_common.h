@@ -101,6 +101,17 @@ __device__ __forceinline__ float wave_sum(float v) {
     return lane63(v);
 }
 
+// sum over aligned groups of LPR lanes, in each of them
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (LPR >= 2) v += dpp<0xb1, 0xf>(0.f, v);       // lane ^ 1
+    if constexpr (LPR >= 4) v += dpp<0x4e, 0xf>(0.f, v);       // lane ^ 2
+    if constexpr (LPR >= 8) v += dpp<0x141, 0xf>(0.f, v);      // the other four of eight
+    if constexpr (LPR >= 16) v += dpp<0x140, 0xf>(0.f, v);     // the other eight of sixteen
+    if constexpr (LPR >= 32) v += __shfl_xor(v, 16);
+    return v;
+}
+
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp<0x111, 0xf>(v, v));
     v = fmaxf(v, dpp<0x112, 0xf>(v, v));

@@ -170,6 +170,7 @@ __device__ __forceinline__ Sums group_sums(Sums s, float c2, float* scratch) {
 }
 
 constexpr int SC_UNROLL = 2;             // pieces of 16 bytes in flight a thread
+constexpr int SC_BWD_UNROLL = 4;         // ... in the backward, which computes less and has no state to keep
 constexpr int SC_BUF = 512;              // candidates for the alternatives
 constexpr int SC_FEW = 128;              // so few scores are all candidates
 
@@ -698,15 +699,16 @@ static int launch_scores(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
 
 // The gradient of a slice of a row: p's part of it everywhere, then the listed ids' values again with what they add.  The first
 // slot of an id adds up all of them in order, so nothing depends on who comes first.  NW waves a slice; NW = 1: four rows a block.
-// List of a group in LDS: n4 ids (padded with -1 to whole fours), then n4 addends.
+// List of a group in LDS: n16 ids (padded with -1 to whole sixteens), then n16 addends.  The first pieces and the list are on their
+// way at the same time.
 template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
-    constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
+    constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_BWD_UNROLL;
     extern __shared__ int4 lists[];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x & (NT - 1), lane = tid & (WAVE - 1);
-    const int n4 = (a.n_ids + 3) & ~3;
-    int32_t* s_id = (int32_t*)lists + group * 2 * n4;
-    float* s_g = (float*)(s_id + n4);
+    const int n16 = (a.n_ids + 15) & ~15;
+    int32_t* s_id = (int32_t*)lists + group * 2 * n16;
+    float* s_g = (float*)(s_id + n16);
     const int64_t units = a.rows * a.splits;
     for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
         const int64_t r = a.splits == 1 ? unit : unit / a.splits;
@@ -715,12 +717,23 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         const int nvec = n / V, rem = n - nvec * V;
         const T* x = row_ptr<T>(a.x, r) + from;
         T* dx = (T*)a.dx + r * a.c + from;
+        u32x4 raw[U];
+        auto load = [&](int j) {                        // past the end: the last piece again
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int at = j + tid + i * NT;
+                if (j + i * NT < nvec) raw[i] = Piece<T>::load(x + (int64_t)(at < nvec ? at : nvec - 1) * V);
+            }
+        };
+        load(0);
         const float m = a.stats[(DISTILL ? 4 : 2) * r], l2 = a.stats[(DISTILL ? 4 : 2) * r + 1];
         const float mt = DISTILL ? a.stats[4 * r + 2] : 0.f, lt = DISTILL ? a.stats[4 * r + 3] : 0.f;
         const bool none = l2 == INFINITY;
         group_sync<NW>();                               // the slice before is done with the list
         float sum = 0.f;
-        for (int k0 = 0; k0 < n4; k0 += WAVE) {         // every wave adds up the whole list, each keeps its share of it
+        int32_t first = -1;                             // this thread's slot of the list (k = tid), its addend and the row's score
+        float first_g = 0.f, first_x = 0.f;
+        for (int k0 = 0; k0 < n16; k0 += WAVE) {        // every wave adds up the whole list, each keeps its share of it
             const int k = k0 + lane;
             int32_t at = -1;
             float g = 0.f;
@@ -735,9 +748,14 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
                 }
                 if (in && id >= from && id < from + n) at = (int32_t)id - from;
             }
-            if (k < n4 && (k0 / WAVE) % NW == tid / WAVE) {
+            if (k < n16 && (k0 / WAVE) % NW == tid / WAVE) {
                 s_id[k] = at;
                 s_g[k] = g;
+                if (k == tid) {
+                    first = at;
+                    first_g = g;
+                    if (at >= 0) first_x = to_f32(x[at]);
+                }
             }
         }
         // dx = p (A + B (log2 p + H2)) + u * (what the listed ids add)
@@ -758,32 +776,16 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
             const float p = exp2_raw(lp);
             return ENT ? p * fmaf(B, fmaxf(lp, Z_FLOOR) + H2, A) : p * A;
         };
-        int64_t j = tid;
-        for (; j - tid + U * NT <= nvec; j += U * NT) {
-            u32x4 raw[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) raw[i] = Piece<T>::load(x + (j + i * NT) * V);
+        for (int j = 0; j < nvec; j += U * NT) {
+            if (j) load(j);
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                float v[V];
-                Piece<T>::unpack(raw[i], v);
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = base(v[e]);
-                Piece<T>::store(dx + (j + i * NT) * V, Piece<T>::pack(v));
-            }
-        }
-        if (j - tid < nvec) {
-            u32x4 raw[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) raw[i] = Piece<T>::load(x + (j + i * NT < nvec ? j + i * NT : nvec - 1) * V);
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (j + i * NT < nvec) {
+                if (j + tid + i * NT < nvec) {
                     float v[V];
                     Piece<T>::unpack(raw[i], v);
 #pragma unroll
                     for (int e = 0; e < V; ++e) v[e] = base(v[e]);
-                    Piece<T>::store(dx + (j + i * NT) * V, Piece<T>::pack(v));
+                    Piece<T>::store(dx + (int64_t)(j + tid + i * NT) * V, Piece<T>::pack(v));
                 }
             }
         }
@@ -793,31 +795,47 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         group_sync<NW>();
         for (int k = tid; k < a.n_ids; k += NT) {
-            const int32_t id = s_id[k];
+            if (k != tid) {
+                first = s_id[k];
+                if (first >= 0) {
+                    first_g = s_g[k];
+                    first_x = to_f32(x[first]);
+                }
+            }
+            const int32_t id = first;
             if (id < 0) continue;
-            float g = s_g[k];
+            float g = first_g;
             int same = 0;
-            for (int i = 0; i < n4; i += 4) {
-                const int4 o = *(const int4*)(s_id + i);
-                same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+            for (int i = 0; i < n16; i += 16)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int4 o = *(const int4*)(s_id + i + 4 * q);
+                    same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+                }
+            if (same > 1) {                             // the first of them adds them all up, in order
+                int lead = k;
+                g = 0.f;
+                for (int i = 0; i < n16; i += 16)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const bool is = s_id[i + q] == id;
+                        lead = is && i + q < lead ? i + q : lead;
+                        g += is ? s_g[i + q] : 0.f;
+                    }
+                if (lead != k) continue;
             }
-            if (same > 1) {
-                bool first = true;
-                for (int i = 0; i < k; ++i) first = first && s_id[i] != id;
-                if (!first) continue;
-                for (int i = k + 1; i < a.n_ids; ++i) g += s_id[i] == id ? s_g[i] : 0.f;
-            }
-            dx[id] = from_f32<T>(fmaf(g, u, base(to_f32(x[id]))));
+            dx[id] = from_f32<T>(fmaf(g, u, base(first_x)));
         }
     }
 }
 
 template <typename T, bool ENT, bool DISTILL>
 static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
-    const bool narrow = a.c <= WAVE * Piece<T>::N * 4;
-    // slices of at most 65536 scores; few rows: down to what a block's threads load at once
-    const int64_t at_once = SC_TPB * Piece<T>::N * SC_UNROLL;
-    int64_t splits = (a.c + 65535) / 65536;
+    const bool narrow = a.c <= WAVE * Piece<T>::N * 4;               // a wave a row: its lanes hold it in one go
+    // slices of 16384 scores (2048 x 131072 bf16: 8192 220 us, 16384 193, 32768 211, 65536 222); few rows: down to what a block's
+    // threads load at once
+    const int64_t at_once = SC_TPB * Piece<T>::N * SC_BWD_UNROLL;
+    int64_t splits = (a.c + 16383) / 16384;
     if (a.rows < 2048) {
         int64_t want = (2048 + a.rows - 1) / a.rows;
         if (want > (a.c + at_once - 1) / at_once) want = (a.c + at_once - 1) / at_once;
@@ -826,7 +844,7 @@ static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
     if (narrow) splits = 1;
     a.per = splits == 1 ? a.c : ((a.c + splits - 1) / splits + 63) / 64 * 64;
     a.splits = (int)((a.c + a.per - 1) / a.per);
-    const size_t list = (size_t)((a.n_ids + 3) & ~3) * 8;
+    const size_t list = (size_t)((a.n_ids + 15) & ~15) * 8;
     if (narrow)
         score_bwd_kernel<T, 1, ENT, DISTILL><<<row_grid((a.rows + 3) / 4), SC_TPB, 4 * list, st>>>(a);
     else
