@@ -39,12 +39,6 @@ struct NormArgs {
     int blocks;
 };
 
-__device__ __forceinline__ float load_param(const void* p, int type, int i) {
-    if (type == ARMNET_F32) return ((const float*)p)[i];
-    if (type == ARMNET_BF16) return (float)((const bf16_t*)p)[i];
-    return (float)((const f16_t*)p)[i];
-}
-
 __device__ __forceinline__ void store_param(void* p, int type, int i, float v) {
     if (type == ARMNET_F32) ((float*)p)[i] = v;
     else if (type == ARMNET_BF16) ((bf16_t*)p)[i] = (bf16_t)v;
@@ -368,25 +362,104 @@ __global__ void __launch_bounds__(LN_SUM_WAVES * WAVE) norm_param_kernel(const f
 
 // ---- rows longer than LN_MAX_D: a block a row, read again for each step ---------------------------------------------------
 
+constexpr int LN_LONG_TPB = 1024, LN_LONG_NW = LN_LONG_TPB / WAVE;
+
+// n elements of a piece, 0 for the others
 template <typename T>
-__global__ void __launch_bounds__(LN_TPB) norm_long_fwd_kernel(NormArgs a) {
-    __shared__ float scratch[LN_TPB / WAVE];
+__device__ __forceinline__ void load_n(const T* p, int n, float (&f)[Piece<T>::N]) {
+    if (n == Piece<T>::N) {
+        Piece<T>::unpack(Piece<T>::load(p), f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < Piece<T>::N; ++e) f[e] = e < n ? to_f32(p[e]) : 0.f;
+    }
+}
+
+// f(elements, first column, how many of them) for the pieces of a row of d elements that this thread owns
+template <typename T, typename F>
+__device__ __forceinline__ void for_pieces(const T* x, int d, F f) {
+    constexpr int V = Piece<T>::N;
+    const int nvec = d / V;
+    int j = threadIdx.x;
+    for (; j + 3 * LN_LONG_TPB < nvec; j += 4 * LN_LONG_TPB) {
+        u32x4 raw[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) raw[u] = Piece<T>::load(x + (int64_t)(j + u * LN_LONG_TPB) * V);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float v[V];
+            Piece<T>::unpack(raw[u], v);
+            f(v, (j + u * LN_LONG_TPB) * V, V);
+        }
+    }
+    for (; j <= nvec; j += LN_LONG_TPB) {
+        const int n = j < nvec ? V : d - nvec * V;
+        if (n == 0) break;
+        float v[V];
+        load_n(x + (int64_t)j * V, n, v);
+        f(v, j * V, n);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_n(T* p, int n, const float (&f)[Piece<T>::N]) {
+    if (n == Piece<T>::N) {
+        Piece<T>::store(p, Piece<T>::pack(f));
+    } else {
+#pragma unroll
+        for (int e = 0; e < Piece<T>::N; ++e)
+            if (e < n) p[e] = from_f32<T>(f[e]);
+    }
+}
+
+// n of a parameter's values from column `at` on, `fill` without one
+template <int V>
+__device__ __forceinline__ void load_params(const void* p, int type, int at, int n, float fill, float (&f)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = fill;
+    if (!p) return;
+    if (type == ARMNET_F32) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = ((const float*)p)[at + (e < n ? e : 0)];
+    } else if (type == ARMNET_BF16) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = to_f32(((const bf16_t*)p)[at + (e < n ? e : 0)]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = to_f32(((const f16_t*)p)[at + (e < n ? e : 0)]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LN_LONG_TPB) norm_long_fwd_kernel(NormArgs a) {
+    constexpr int V = Piece<T>::N;
+    __shared__ float scratch[LN_LONG_NW];
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = row_ptr<T>(a.x, r);
-        float s = 0.f;
-        for (int i = threadIdx.x; i < a.d; i += LN_TPB) s += to_f32(x[i]);
-        const float mean = block_sum<LN_TPB / WAVE>(s, scratch) / (float)a.d;
-        float q = 0.f;
-        for (int i = threadIdx.x; i < a.d; i += LN_TPB) {
-            const float c = to_f32(x[i]) - mean;
-            q = fmaf(c, c, q);
-        }
-        const float rstd = 1.f / sqrtf(block_sum<LN_TPB / WAVE>(q, scratch) / (float)a.d + a.eps);
         T* y = (T*)a.out + r * a.d;
-        for (int i = threadIdx.x; i < a.d; i += LN_TPB) {
-            const float w = a.weight ? load_param(a.weight, a.w_type, i) : 1.f, b = a.bias ? load_param(a.bias, a.w_type, i) : 0.f;
-            y[i] = from_f32<T>(fmaf((to_f32(x[i]) - mean) * rstd, w, b));
-        }
+        float s = 0.f;
+        for_pieces(x, a.d, [&](const float (&v)[V], int, int) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += v[e];
+        });
+        const float mean = block_sum<LN_LONG_NW>(s, scratch) / (float)a.d;
+        float q = 0.f;
+        for_pieces(x, a.d, [&](const float (&v)[V], int, int n) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float c = e < n ? v[e] - mean : 0.f;
+                q = fmaf(c, c, q);
+            }
+        });
+        const float rstd = 1.f / sqrtf(block_sum<LN_LONG_NW>(q, scratch) / (float)a.d + a.eps);
+        for_pieces(x, a.d, [&](const float (&v)[V], int at, int n) {
+            float o[V], w[V], b[V];
+            load_params(a.weight, a.w_type, at, n, 1.f, w);
+            load_params(a.bias, a.w_type, at, n, 0.f, b);
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = fmaf((v[e] - mean) * rstd, w[e], b[e]);
+            store_n(y + at, n, o);
+        });
         if (threadIdx.x == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -395,26 +468,43 @@ __global__ void __launch_bounds__(LN_TPB) norm_long_fwd_kernel(NormArgs a) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LN_TPB) norm_long_dx_kernel(NormArgs a) {
-    __shared__ float scratch[LN_TPB / WAVE];
+__global__ void __launch_bounds__(LN_LONG_TPB) norm_long_dx_kernel(NormArgs a) {
+    constexpr int V = Piece<T>::N;
+    __shared__ float scratch[LN_LONG_NW];
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = row_ptr<T>(a.x, r);
         const T* dy = (const T*)a.dy + r * a.d;
+        T* dx = (T*)a.out + r * a.d;
         const float mean = a.mean[r], rstd = a.rstd[r];
         float s1 = 0.f, s2 = 0.f;
-        for (int i = threadIdx.x; i < a.d; i += LN_TPB) {
-            const float g = to_f32(dy[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
-            s1 += g;
-            s2 = fmaf(g, (to_f32(x[i]) - mean) * rstd, s2);
-        }
-        const float m1 = block_sum<LN_TPB / WAVE>(s1, scratch) / (float)a.d;
-        const float m2 = block_sum<LN_TPB / WAVE>(s2, scratch) / (float)a.d;
-        T* dx = (T*)a.out + r * a.d;
-        for (int i = threadIdx.x; i < a.d; i += LN_TPB) {
-            const float g = to_f32(dy[i]) * (a.weight ? load_param(a.weight, a.w_type, i) : 1.f);
-            const float h = (to_f32(x[i]) - mean) * rstd;
-            dx[i] = from_f32<T>(rstd * (g - m1 - h * m2));
-        }
+        auto both = [&](const float (&v)[V], int at, int n, float (&g)[V], float (&h)[V]) {
+            float w[V];
+            load_n(dy + at, n, g);                     // 0 past the end
+            load_params(a.weight, a.w_type, at, n, 1.f, w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                g[e] *= w[e];
+                h[e] = (v[e] - mean) * rstd;
+            }
+        };
+        for_pieces(x, a.d, [&](const float (&v)[V], int at, int n) {
+            float g[V], h[V];
+            both(v, at, n, g, h);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s1 += g[e];
+                s2 = fmaf(g[e], h[e], s2);
+            }
+        });
+        const float m1 = block_sum<LN_LONG_NW>(s1, scratch) / (float)a.d;
+        const float m2 = block_sum<LN_LONG_NW>(s2, scratch) / (float)a.d;
+        for_pieces(x, a.d, [&](const float (&v)[V], int at, int n) {
+            float g[V], h[V];
+            both(v, at, n, g, h);
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] = rstd * (g[e] - m1 - h[e] * m2);
+            store_n(dx + at, n, g);
+        });
     }
 }
 
@@ -427,6 +517,7 @@ __global__ void __launch_bounds__(LN_TPB) norm_long_param_kernel(NormArgs a) {
     const int64_t r0 = blockIdx.y * per;
     const int64_t r1 = r0 + per < a.rows ? r0 + per : a.rows;
     float sw = 0.f, sb = 0.f;
+#pragma unroll 4
     for (int64_t r = r0; r < r1; ++r) {
         const float g = to_f32(((const T*)a.dy)[r * a.d + i]);
         sw = fmaf(g, (to_f32(row_ptr<T>(a.x, r)[i]) - a.mean[r]) * a.rstd[r], sw);
@@ -553,7 +644,7 @@ int armnet_layer_norm_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int
         ARMNET_ROW_TYPE(x_type, T, there = launch_norm_fwd<T>(a, st));
         if (!there) return ARMNET_ERR_UNSUPPORTED;
     } else {
-        ARMNET_ROW_TYPE(x_type, T, (norm_long_fwd_kernel<T><<<row_grid(rows), LN_TPB, 0, st>>>(a)));
+        ARMNET_ROW_TYPE(x_type, T, (norm_long_fwd_kernel<T><<<row_grid(rows), LN_LONG_TPB, 0, st>>>(a)));
     }
     ARMNET_LAUNCH_CHECK();
     return ARMNET_OK;
@@ -591,7 +682,7 @@ int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int
             if (a.blocks == 1) return ARMNET_OK;                     // the one block has written the parameters' gradients
         } else {
             if (dx) {
-                ARMNET_ROW_TYPE(x_type, T, (norm_long_dx_kernel<T><<<row_grid(rows), LN_TPB, 0, st>>>(a)));
+                ARMNET_ROW_TYPE(x_type, T, (norm_long_dx_kernel<T><<<row_grid(rows), LN_LONG_TPB, 0, st>>>(a)));
                 ARMNET_LAUNCH_CHECK();
             }
             if (params) {

@@ -112,6 +112,16 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+template <int LPR>
+__device__ __forceinline__ float lanes_max(float v) {
+    if constexpr (LPR >= 2) v = fmaxf(v, dpp<0xb1, 0xf>(v, v));
+    if constexpr (LPR >= 4) v = fmaxf(v, dpp<0x4e, 0xf>(v, v));
+    if constexpr (LPR >= 8) v = fmaxf(v, dpp<0x141, 0xf>(v, v));
+    if constexpr (LPR >= 16) v = fmaxf(v, dpp<0x140, 0xf>(v, v));
+    if constexpr (LPR >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+    return v;
+}
+
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp<0x111, 0xf>(v, v));
     v = fmaxf(v, dpp<0x112, 0xf>(v, v));

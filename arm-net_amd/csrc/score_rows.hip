@@ -637,6 +637,290 @@ __global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
     }
 }
 
+// ---- short rows: LPR lanes of a wave a row -------------------------------------------------------------------------------
+//
+// What a row costs beside reading it — maxima and sums across lanes, the ids, the writes — is the same instructions for one row or
+// for the 64 / LPR rows that a wave holds side by side.  A lane keeps P pieces; the piece that crosses the row's end is pulled
+// back into it, as in layer_norm.hip.
+
+template <typename T, int LPR, int P>
+struct ShortRow {
+    static constexpr int V = Piece<T>::N;
+    float v[P][V];
+    int off[P], lo[P];                    // the lane's own: columns off + e for e in [lo, V)
+    __device__ __forceinline__ void load(const T* x, int c, int tid) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int at = (i * LPR + tid) * V;
+            if (c >= V) {
+                off[i] = at + V <= c ? at : c - V;
+                lo[i] = at - off[i] < V ? at - off[i] : V;
+                Piece<T>::unpack(Piece<T>::load(x + off[i]), v[i]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[i][e] = e >= lo[i] ? v[i][e] : -INFINITY;
+            } else {                      // the first lane holds all: columns c - V .. c - 1, of which the negative are not there
+                off[i] = c - V;
+                lo[i] = at ? V : V - c;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[i][e] = e >= lo[i] ? to_f32(x[off[i] + e]) : -INFINITY;
+            }
+        }
+    }
+};
+
+// keys of (value, lowest column first) of a short row.  A 16-bit score is exact in the upper 19 bits of its fp32 form, which leaves 13
+// for the column and halves what a comparison costs.  Of a masked score only the column remains.
+template <typename T>
+struct ShortKey {
+    typedef uint64_t type;
+    static __device__ __forceinline__ type of(float v, uint32_t col) { return v > -INFINITY ? score_key(v, col) : (type)~col; }
+    static __device__ __forceinline__ bool live(type k) { return k >> 32; }
+};
+struct ShortKey16 {
+    typedef uint32_t type;
+    static __device__ __forceinline__ type of(float v, uint32_t col) {
+        return (v > -INFINITY ? value_key(v) & ~0x1fffu : 0u) | (0x1fffu - col);
+    }
+    static __device__ __forceinline__ bool live(type k) { return k >> 13; }
+};
+template <>
+struct ShortKey<bf16_t> : ShortKey16 {};
+template <>
+struct ShortKey<f16_t> : ShortKey16 {};
+
+template <typename T, int LPR, int P, bool ENT, bool TOP, bool DISTILL>
+__global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
+    typedef ShortKey<T> Key;
+    constexpr int V = Piece<T>::N, ROWS = SC_TPB / LPR, W = TOP ? LPR * P * V + 1 : 1;
+    __shared__ typename Key::type keys[TOP ? ROWS * W : 1];
+    const int tid = threadIdx.x & (LPR - 1), slot = threadIdx.x / LPR;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * ROWS) {
+        const bool in = r0 + slot < a.rows;            // lanes without a row work on the last one's and write nothing
+        const int64_t r = in ? r0 + slot : a.rows - 1;
+        const T* x = row_ptr<T>(a.x, r);
+        int64_t id = -1;
+        if (tid < a.n_ids) id = load_id(a.ids, a.id_type, r * a.n_ids + tid);
+        ShortRow<T, LPR, P> row;
+        row.load(x, a.c, tid);
+        Sums s{-FLT_MAX, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s.m = fmaxf(s.m, row.v[i][e]);
+        s.m = lanes_max<LPR>(s.m);
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float z = (row.v[i][e] - s.m) * a.c2, p = exp2_raw(z);
+                s.S += p;
+                if constexpr (ENT) s.W = fmaf(p, fmaxf(z, Z_FLOOR), s.W);
+            }
+        s.S = lanes_sum<LPR>(s.S);
+        if constexpr (ENT) s.W = lanes_sum<LPR>(s.W);
+        const bool some = !(s.S == 0.f);
+        const float l2 = some ? log2f(s.S) : INFINITY;
+        if constexpr (!DISTILL) {
+            if (in && tid == 0) {
+                if (ENT) a.entropy[r] = some ? LN2 * (l2 - s.W / s.S) : 0.f;
+                if (a.stats) {
+                    a.stats[2 * r] = s.m;
+                    a.stats[2 * r + 1] = l2;
+                }
+            }
+            for (int k = tid; k < a.n_ids; k += LPR) {
+                if (k != tid) id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                float v = 0.f;
+                if (id >= a.c) {
+                    v = NAN;
+                    if (a.id_status) flag_bad_id(a.id_status);
+                } else if (id >= 0) {
+                    v = some ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : -INFINITY;
+                }
+                if (in) a.logp[r * a.n_ids + k] = v;
+            }
+        } else {
+            float mt = -FLT_MAX, st = 0.f, loss = 0.f;
+            for (int k = tid; k < a.n_ids; k += LPR) {
+                id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                if (id >= 0) mt = fmaxf(mt, load_any(a.teacher, a.t_type, r * a.n_ids + k));
+                if (id >= a.c && a.id_status) flag_bad_id(a.id_status);
+            }
+            mt = lanes_max<LPR>(mt);
+            for (int k = tid; k < a.n_ids; k += LPR)
+                if (load_id(a.ids, a.id_type, r * a.n_ids + k) >= 0)
+                    st += exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2);
+            st = lanes_sum<LPR>(st);
+            const float lt = st == 0.f ? INFINITY : log2f(st);
+            for (int k = tid; k < a.n_ids; k += LPR) {
+                id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                if (id < 0) continue;
+                const float zt = load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt;
+                const float q = exp2_raw(zt * a.c2 - lt);
+                const float lp = id < a.c ? (to_f32(x[id]) - s.m) * a.rt - LN2 * l2 : NAN;
+                if (!(q == 0.f)) loss = fmaf(q, (zt * a.rt - LN2 * lt) - lp, loss);
+            }
+            loss = lanes_sum<LPR>(loss) * (a.t * a.t);
+            if (in && tid == 0) {
+                a.loss[r] = loss;
+                if (a.stats) {
+                    a.stats[4 * r + 0] = s.m;
+                    a.stats[4 * r + 1] = l2;
+                    a.stats[4 * r + 2] = mt;
+                    a.stats[4 * r + 3] = lt;
+                }
+            }
+        }
+        if constexpr (TOP) {                           // a score's rank: how many of the row are better
+            typename Key::type* mine = keys + slot * W;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e >= row.lo[i]) {
+                        const uint32_t col = row.off[i] + e;
+                        mine[col] = Key::of(row.v[i][e], col);
+                    }
+            group_sync<1>();
+            typename Key::type key[P][V];
+            int rank[P][V] = {};
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) key[i][e] = e >= row.lo[i] ? mine[row.off[i] + e] : 0;
+            for (int j = 0; j < a.c; ++j) {
+                const typename Key::type other = mine[j];
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) rank[i][e] += other > key[i][e] ? 1 : 0;
+            }
+            const bool nan = s.S != s.S;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (in && e >= row.lo[i] && rank[i][e] < a.top) {
+                        const bool live = !nan && Key::live(key[i][e]);
+                        a.top_ids[r * a.top + rank[i][e]] = live ? row.off[i] + e : -1;
+                        a.top_logp[r * a.top + rank[i][e]] = nan ? NAN : live ? (row.v[i][e] - s.m) * a.rt - LN2 * l2 : -INFINITY;
+                    }
+            group_sync<1>();
+        }
+    }
+}
+
+// the gradient; what the listed ids add is summed per column in LDS, slot after slot
+template <typename T, int LPR, int P, bool ENT, bool DISTILL>
+__global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
+    constexpr int V = Piece<T>::N, ROWS = SC_TPB / LPR;
+    extern __shared__ float added[];                   // [ROWS, c]
+    const int tid = threadIdx.x & (LPR - 1), slot = threadIdx.x / LPR;
+    float* mine = added + slot * a.c;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * ROWS) {
+        const bool in = r0 + slot < a.rows;
+        const int64_t r = in ? r0 + slot : a.rows - 1;
+        const T* x = row_ptr<T>(a.x, r);
+        ShortRow<T, LPR, P> row;
+        row.load(x, a.c, tid);
+        const float m = a.stats[(DISTILL ? 4 : 2) * r], l2 = a.stats[(DISTILL ? 4 : 2) * r + 1];
+        const float mt = DISTILL ? a.stats[4 * r + 2] : 0.f, lt = DISTILL ? a.stats[4 * r + 3] : 0.f;
+        const bool none = l2 == INFINITY;
+        for (int i = tid; i < a.c; i += LPR) mine[i] = 0.f;
+        group_sync<1>();
+        float sum = 0.f;
+        for (int k0 = 0; k0 < a.n_ids; k0 += LPR) {
+            int at = -1;
+            float g = 0.f;
+            if (k0 + tid < a.n_ids) {
+                const int64_t k = r * a.n_ids + k0 + tid, id = load_id(a.ids, a.id_type, k);
+                if (id >= 0 && id < a.c && !none) {
+                    at = (int)id;
+                    if (DISTILL) g = exp2_raw((load_any(a.teacher, a.t_type, k) - mt) * a.c2 - lt);
+                    else if (a.g_logp) g = a.g_logp[k];
+                    sum += g;
+                }
+            }
+            const int slots = a.n_ids - k0 < LPR ? a.n_ids - k0 : LPR;
+            for (int t = 0; t < slots; ++t) {
+                if (tid == t && at >= 0) mine[at] += g;
+                group_sync<1>();
+            }
+        }
+        group_sync<1>();
+        float A, B = 0.f, H2 = 0.f, u;
+        if (DISTILL) {
+            u = -a.g_logp[r] * a.t;
+            A = lt == INFINITY ? 0.f : -u + (lt - lt);
+        } else {
+            A = -lanes_sum<LPR>(sum) * a.rt;
+            u = a.rt;
+            if (ENT) {
+                B = -a.g_entropy[r] * LN2 * a.rt;
+                H2 = a.entropy[r] / LN2;
+            }
+        }
+        T* dx = (T*)a.dx + r * a.c;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float lp = fmaf(row.v[i][e] - m, a.c2, -l2);
+                const float p = exp2_raw(lp);
+                const float d = ENT ? p * fmaf(B, fmaxf(lp, Z_FLOOR) + H2, A) : p * A;
+                o[e] = e >= row.lo[i] ? fmaf(mine[row.off[i] + e], u, d) : 0.f;
+            }
+            if (!in) continue;
+            if (row.lo[i] == 0) {
+                Piece<T>::store(dx + row.off[i], Piece<T>::pack(o));
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e >= row.lo[i]) dx[row.off[i] + e] = from_f32<T>(o[e]);
+            }
+        }
+        group_sync<1>();
+    }
+}
+
+static unsigned short_grid(int64_t rows, int lpr) {
+    const int64_t blocks = (rows * lpr + SC_TPB - 1) / SC_TPB, most = (int64_t)device_cu_count() * 8;
+    return (unsigned)(blocks < most ? blocks : most);
+}
+
+// Rows this short go several to a wave: 4 lanes with up to four pieces each, or 16.  With alternatives every score of a row is
+// compared with every other: up to 64 of them, 8 or less a lane.
+template <typename T, bool ENT, bool TOP, bool DISTILL>
+static bool launch_short_fwd(const ScoreArgs& a, hipStream_t st) {
+    constexpr int V = Piece<T>::N;
+    if (DISTILL && a.n_ids > 64) return false;
+    if constexpr (TOP) {
+        constexpr int P = sizeof(T) == 4 ? 2 : 1;
+        if (a.c <= 4 * P * V) score_short_fwd_kernel<T, 4, P, ENT, true, false><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 64) score_short_fwd_kernel<T, 64 / V, 1, ENT, true, false><<<short_grid(a.rows, 64 / V), SC_TPB, 0, st>>>(a);
+        else return false;
+    } else {
+        if (a.c <= 4 * V) score_short_fwd_kernel<T, 4, 1, ENT, false, DISTILL><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 16 * V) score_short_fwd_kernel<T, 16, 1, ENT, false, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 64 * V) score_short_fwd_kernel<T, 16, 4, ENT, false, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
+        else return false;
+    }
+    return true;
+}
+
+template <typename T, bool ENT, bool DISTILL>
+static bool launch_short_bwd(const ScoreArgs& a, hipStream_t st) {
+    constexpr int V = Piece<T>::N;
+    if (a.n_ids > 64) return false;
+    const size_t row = (size_t)a.c * sizeof(float);
+    if (a.c <= 4 * V) score_short_bwd_kernel<T, 4, 1, ENT, DISTILL><<<short_grid(a.rows, 4), SC_TPB, SC_TPB / 4 * row, st>>>(a);
+    else if (a.c <= 16 * V) score_short_bwd_kernel<T, 16, 1, ENT, DISTILL><<<short_grid(a.rows, 16), SC_TPB, SC_TPB / 16 * row, st>>>(a);
+    else if (a.c <= 64 * V) score_short_bwd_kernel<T, 16, 4, ENT, DISTILL><<<short_grid(a.rows, 16), SC_TPB, SC_TPB / 16 * row, st>>>(a);
+    else return false;
+    return true;
+}
+
 // Slices of a row: what makes rounds(slices) * (a slice's length + what a slice costs beside reading it) + the joining kernel
 // smallest.  The costs are in scores that a block of a full chip reads meanwhile (2.7 KB/us of 16-bit scores): about 2 us a slice,
 // 5 us with alternatives, 5 us for the second kernel.  No slice is below 4096 scores; the joining kernel has a thread for each.
@@ -668,6 +952,10 @@ static int64_t score_ws(int64_t rows, int64_t c, int top) {
 
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 static int launch_score_fwd(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+    if (launch_short_fwd<T, ENT, TOP, DISTILL>(a, st)) {
+        ARMNET_LAUNCH_CHECK();
+        return ARMNET_OK;
+    }
     a.splits = score_splits(a.rows, a.c, a.top);
     a.per = a.splits == 1 ? a.c : ((a.c + a.splits - 1) / a.splits + 63) / 64 * 64;
     if (a.splits > 1) {
@@ -831,6 +1119,10 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
 
 template <typename T, bool ENT, bool DISTILL>
 static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
+    if (launch_short_bwd<T, ENT, DISTILL>(a, st)) {
+        ARMNET_LAUNCH_CHECK();
+        return ARMNET_OK;
+    }
     const bool narrow = a.c <= WAVE * Piece<T>::N * 4;               // a wave a row: its lanes hold it in one go
     // slices of 16384 scores (2048 x 131072 bf16: 8192 220 us, 16384 193, 32768 211, 65536 222); few rows: down to what a block's
     // threads load at once

@@ -272,6 +272,26 @@ def test_score_gradients_masks(c, dtype):
     assert got[2].eq(0).all() and got[4].isnan().all() and not got[[0, 1, 3, 5]].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,c", [(70001, 2), (40007, 10), (20001, 33), (9001, 64), (5003, 250), (4999, 2050), (4100, 5382)])
+def test_many_rows(n, c, dtype):
+    """several rows a wave, a wave a row, more rows than the launch has waves"""
+    x = (rnd(n, c) * 2).to(dtype)
+    x[n - 1, c // 2:] = -INF
+    x[7] = -INF
+    ids = torch.randint(-1, c, (n, 2), generator=gen(1))
+    check_scores(x, ids, 1.0, min(c, 7))
+    check_scores(x, ids[:, :1], 0.8, 0)
+    xd = x.to(DEV).requires_grad_(True)
+    g, gh = rnd(n, 2, seed=2), rnd(n, seed=3)
+    r = score_logprobs(xd, ids.to(DEV), 1.0, entropy=True)
+    got, = torch.autograd.grad((r.logp, r.entropy), xd, (g.to(DEV), gh.to(DEV)))
+    score_gradients(x, ids, 1.0, g, gh, dtype, got)
+    lesson_ids, ts, up = lesson((n,), c, 3)
+    x[7] = 0
+    check_distill(x, lesson_ids, ts, 2.0, up, dtype)
+
+
 @pytest.mark.parametrize("n", [64, 65, 200, 1024])
 def test_long_lists_of_ids(n):
     """every slot of a long list, most ids several times"""
