@@ -798,7 +798,7 @@ def _score_ids(ids, lead, dev, name):
     """(ids of a row, their type): `ids` [.., n] dense beside rows of the shape `lead`"""
     if ids is None:
         return 0, ID_I64
-    if tuple(ids.shape[:-1]) != tuple(lead) or not ids.is_contiguous() or ids.get_device() != dev:
+    if ids.shape[:-1] != lead or not ids.is_contiguous() or ids.get_device() != dev:
         raise ArmnetNativeError(f"{name}: expected a dense {list(lead) + ['n']} tensor on device {dev}, got {list(ids.shape)} on "
                                 f"{ids.device} (contiguous={ids.is_contiguous()})")
     return ids.shape[-1], _id_type(ids)

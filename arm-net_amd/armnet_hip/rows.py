@@ -49,6 +49,13 @@ def _temperature(t):
     return float(t)
 
 
+def _poll(status, devices):
+    for d in devices:
+        if d.type == "cuda":
+            torch.cuda.synchronize(d)
+    status.raise_if_set()
+
+
 # ---- layer norm ----------------------------------------------------------------------------------------------------------
 
 class _LayerNormFn(torch.autograd.Function):
@@ -154,7 +161,7 @@ def _row_ids(ids, lead, name):
     if ids.dtype not in (torch.int64, torch.int32):
         raise native.ArmnetNativeError(f"{name} must be int64 or int32, got {ids.dtype}")
     one = ids.dim() == len(lead)
-    if tuple(ids.shape if one else ids.shape[:-1]) != tuple(lead) or not 0 <= ids.dim() - len(lead) <= 1:
+    if not 0 <= ids.dim() - len(lead) <= 1 or (ids.shape if one else ids.shape[:-1]) != lead:
         raise native.ArmnetNativeError(f"{name}: expected {list(lead)} or {list(lead) + ['n']}, got {list(ids.shape)}")
     ids = ids.unsqueeze(-1) if one else ids
     if ids.shape[-1] > native.MAX_ROW_IDS:
@@ -207,14 +214,14 @@ class HipScoreLogprobs(nn.Module):
         super().__init__()
         self.temperature, self.top_k, self.entropy = _temperature(temperature), top_k, entropy
         self.check_ids = True
-        self._id_status, self._where = IdStatus(), None
+        self._id_status, self._where = IdStatus(), set()
 
     def poll(self):
         """synchronise and raise IndexError if a call so far met an id past its row"""
-        self._id_status.poll(self._where)
+        _poll(self._id_status, self._where)
 
     def forward(self, X, ids=None):
-        self._where = X.device if X.is_cuda else None
+        self._where.add(X.device)
         return score_logprobs(X, ids, self.temperature, self.top_k, self.entropy, self.check_ids, self._id_status)
 
 
@@ -259,7 +266,7 @@ def distill_loss(X, top_ids, top_scores, temperature=1.0, check_ids=True, status
     ids, one = _row_ids(top_ids, X.shape[:-1], "top_ids")
     if one or ids.shape[-1] < 1:
         raise native.ArmnetNativeError(f"top_ids: expected {list(X.shape[:-1]) + ['k']}, got {list(top_ids.shape)}")
-    if tuple(top_scores.shape) != tuple(ids.shape) or (top_scores.dtype not in _FLOATS and top_scores.dtype != X.dtype):
+    if top_scores.shape != ids.shape or (top_scores.dtype not in _FLOATS and top_scores.dtype != X.dtype):
         raise native.ArmnetNativeError(f"top_scores: expected float32, bfloat16 or float16 of top_ids' shape {list(ids.shape)}, "
                                        f"got {list(top_scores.shape)} {top_scores.dtype}")
     if top_scores.requires_grad and torch.is_grad_enabled():
@@ -293,13 +300,13 @@ class HipDistillLoss(nn.Module):
             raise native.ArmnetNativeError(f"reduction: expected 'mean', 'sum' or 'none', got {reduction!r}")
         self.temperature, self.reduction = _temperature(temperature), reduction
         self.check_ids = True
-        self._id_status, self._where = IdStatus(), None
+        self._id_status, self._where = IdStatus(), set()
 
     def poll(self):
         """synchronise and raise IndexError if a call so far met an id past its row"""
-        self._id_status.poll(self._where)
+        _poll(self._id_status, self._where)
 
     def forward(self, X, top_ids, top_scores):
-        self._where = X.device if X.is_cuda else None
+        self._where.add(X.device)
         loss = distill_loss(X, top_ids, top_scores, self.temperature, self.check_ids, self._id_status)
         return loss if self.reduction == "none" else getattr(loss, self.reduction)()

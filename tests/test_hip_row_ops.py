@@ -614,3 +614,47 @@ def test_norm_projection_scores_and_distillation_together():
     torch.testing.assert_close(loss.detach().cpu().double(), want.detach(), rtol=1e-5, atol=1e-6)
     for got, ref in ((student.weight.grad, ws.grad), (student.bias.grad, bs.grad), (norm.weight.grad, gamma.grad), (norm.bias.grad, beta.grad)):
         torch.testing.assert_close(got.cpu().double(), ref, rtol=1e-4, atol=1e-5 * float(ref.abs().max()))
+
+
+def test_saved_tensors_that_were_moved():
+    """hooks that keep the saved tensors elsewhere: the backward takes them where they come back, dense"""
+    base = rnd(12, 300).to(DEV)
+    x = base[:, 3:].detach().requires_grad_(True)                # a view with a stride of its own
+    w = rnd(297, seed=1).to(DEV).requires_grad_(True)
+    ids, ts, _ = lesson((12,), 297, 5)
+    ids, ts = ids.to(DEV), ts.to(DEV)
+
+    def grads(out):
+        return torch.autograd.grad(out, (x, w), torch.ones_like(out), allow_unused=True)
+
+    calls = [lambda: layer_norm(x, w), lambda: score_logprobs(x, ids, 1.3, entropy=True).logp,
+             lambda: score_logprobs(x, entropy=True).entropy, lambda: distill_loss(x, ids, ts, 2.0)]
+    for call in calls:
+        want = grads(call())
+        with torch.autograd.graph.save_on_cpu():
+            moved = call()
+        junk = [torch.full_like(base, 7.0) for _ in range(3)]    # whatever freed memory is taken again
+        got = grads(moved)
+        del junk
+        for a, b in zip(got, want):
+            assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+def test_second_backward_of_one_graph():
+    x = rnd(9, 200).to(DEV).requires_grad_(True)
+    ids, ts, g = lesson((9,), 200, 4)
+    loss = distill_loss(x, ids.to(DEV), ts.to(DEV))
+    a, = torch.autograd.grad(loss, x, g.to(DEV), retain_graph=True)
+    b, = torch.autograd.grad(loss, x, 2 * g.to(DEV))
+    assert torch.equal(2 * a, b)
+    y = layer_norm(x)
+    first, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError):
+        first.sum().backward()                                   # differentiable once
+    with torch.no_grad():
+        x.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        y2 = layer_norm(x)
+        with torch.no_grad():
+            x.add_(1)
+        y2.sum().backward()
