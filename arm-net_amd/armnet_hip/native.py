@@ -5,6 +5,7 @@ the product path fails loudly.  Tensors are passed as raw device pointers and
 the current torch HIP stream; PyTorch is used only for memory and streams.
 """
 import ctypes
+import importlib.util
 import os
 import subprocess
 
@@ -19,7 +20,6 @@ ABI_VERSION = 8
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_ID_RANGE, ERR_HIP = 0, -1, -2, -3, -4
 ID_I64, ID_I32 = 0, 1
 ONE_HEAD, MULTI_HEAD, GC_ARM = 0, 1, 2
-F32, BF16, F16 = 0, 1, 2                    # armnet_float_type: element types of the row operators
 MAX_ROW_IDS, MAX_ROW_TOP = 1024, 64         # ids / alternatives of one row of scores
 F_WRITE_CLAMPED_VALS, F_FAITHFUL_BISECT, F_FORCE_GENERIC, F_NO_LIN_FINISH, F_FP32_CONTRACTIONS = 0x1, 0x2, 0x4, 0x8, 0x10
 
@@ -45,24 +45,6 @@ EXPORTS = (
 )
 
 _lib = None
-
-
-def _declare_row_calls(lib):
-    """argument types of the row operators' calls: plain Python numbers and addresses are passed without wrapping each"""
-    i, l, f, p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
-    view = [l, l, l, l, l, i, p]                        # rows, inner, outer_stride, row_stride, last dimension, type, x
-    ids = [f, l, p, i]                                  # temperature, ids of a row, ids, their type
-    for name, args, res in (
-            ("armnet_layer_norm_fwd", view + [i, p, p, f, p, p, p, p], i),
-            ("armnet_layer_norm_bwd_ws_bytes", [l, l], l),
-            ("armnet_layer_norm_bwd", view + [p, i, p, p, p, p, p, p, p, l, p], i),
-            ("armnet_score_ws_bytes", [l, l, i], l),
-            ("armnet_score_logprobs_fwd", view + ids + [i, p, p, p, p, p, p, l, p, p], i),
-            ("armnet_score_logprobs_bwd", view + ids + [p, p, p, p, p, p], i),
-            ("armnet_distill_fwd", view + ids + [i, p, p, p, p, l, p, p], i),
-            ("armnet_distill_bwd", view + ids + [i, p, p, p, p, p], i)):
-        fn = getattr(lib, name)
-        fn.argtypes, fn.restype = args, res
 
 
 class ArmnetNativeError(RuntimeError):
@@ -96,7 +78,6 @@ def load():
     lib.armnet_shard_route_fixed_ws_bytes.restype = ctypes.c_int64
     lib.armnet_last_hip_error.restype = ctypes.c_char_p
     lib.armnet_mlp_packed_bytes.restype = ctypes.c_int64
-    _declare_row_calls(lib)
     if lib.armnet_abi_version() != ABI_VERSION:
         raise ArmnetNativeError(f"ABI version mismatch: library {lib.armnet_abi_version()} != binding {ABI_VERSION}")
     _lib = lib
@@ -677,202 +658,24 @@ def shard_direct_perm(n, ids, R, nfeat, perm, id_status=None):
                                               ctypes.c_int64(nfeat), _ptr(perm), _ptr(id_status), _stream()))
 
 
-# ---- row operators: rows are the last dimension, float32 / bfloat16 / float16 --------------------------------------------
+# ---- row operators (layer norm, log probabilities, distillation) -----------------------------------------------------------
 
-_ROW_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-
-
-def row_type(t, name):
-    try:
-        return _ROW_TYPES[t.dtype]
-    except KeyError:
-        raise ArmnetNativeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}") from None
+ROWS_PATH = os.path.join(_PKG, "lib", "_armnet_rows.so")
+_rows = None
 
 
-def row_view(x):
-    """(x or a dense copy, rows, inner, outer_stride, row_stride): the rows of x as the C calls take them.  Leading dimensions
-    that two strides describe need no copy (slices, transposed batches, expanded rows); neighbours in a row are adjacent."""
-    d = x.shape[-1]
-    if x.is_contiguous():
-        return x, x.numel() // d, 0, 0, d
-    if d == 1 or x.stride(-1) == 1:
-        dims = []
-        for n, st in zip(x.shape[:-1], x.stride()[:-1]):
-            if n == 1:
-                continue
-            if dims and dims[-1][1] == st * n:
-                dims[-1] = (dims[-1][0] * n, st)
-            else:
-                dims.append((n, st))
-        rows = x.numel() // d
-        if len(dims) <= 1:
-            return x, rows, 0, 0, (dims[0][1] if dims else d)
-        if len(dims) == 2:
-            return x, rows, dims[1][0], dims[0][1], dims[1][1]
-    x = x.contiguous()
-    return x, x.numel() // d, 0, 0, d
-
-
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _row_stream(dev):
-    """the current stream of device `dev`, as an address (these calls are short: the Stream object costs more than a launch)"""
-    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
-
-
-def _on_its_device(fn):
-    """run `fn(x, ...)` with x's device as the current one (the library queries it); host tensors raise"""
-    def call(x, *args):
-        if not x.is_cuda:
-            raise ArmnetNativeError(f"expected a tensor on the HIP device, got one on {x.device} (no CPU fallback)")
-        dev = x.get_device()
-        if dev == torch.cuda.current_device():
-            return fn(dev, x, *args)
-        with torch.cuda.device(dev):
-            return fn(dev, x, *args)
-    call.__name__, call.__doc__ = fn.__name__, fn.__doc__
-    return call
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _dense(t, n, dev, name, dtype):
-    """`t` (or None) is n adjacent elements of dtype on device dev"""
-    if t is not None and not (t.is_contiguous() and t.numel() == n and t.dtype == dtype and t.get_device() == dev):
-        raise ArmnetNativeError(f"{name}: expected {n} adjacent elements of {dtype} on device {dev}, got {list(t.shape)} "
-                                f"{t.dtype} on {t.device} (contiguous={t.is_contiguous()})")
-
-
-def _like(x):
-    """a new dense tensor of x's shape, type and device"""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-
-
-@_on_its_device
-def layer_norm_fwd(dev, x, weight, bias, eps, stats):
-    """armnet_layer_norm_fwd(x, weight, bias, eps, stats): (y, statistics [2, rows] for the backward or None)"""
-    x, rows, inner, so, sr = row_view(x)
-    d = x.shape[-1]
-    p = weight if weight is not None else bias
-    if p is not None:
-        _dense(weight, d, dev, "weight", p.dtype)
-        _dense(bias, d, dev, "bias", p.dtype)
-    y = _like(x)
-    st = mean = rstd = None
-    if stats:
-        st = torch.empty((2, rows), device=x.device, dtype=torch.float32)
-        mean = st.data_ptr()
-        rstd = mean + 4 * rows
-    if rows:
-        check(load().armnet_layer_norm_fwd(rows, inner, so, sr, d, row_type(x, "x"), x.data_ptr(),
-                                           F32 if p is None else row_type(p, "weight"), _addr(weight), _addr(bias), eps,
-                                           y.data_ptr(), mean, rstd, _row_stream(dev)))
-    return y, st
-
-
-@_on_its_device
-def layer_norm_bwd(dev, x, dy, weight, st, need_dx, need_dw, need_db, p_dtype):
-    """armnet_layer_norm_bwd(x, dy, weight, statistics, ...): (dx, dweight, dbias), None where not needed; the parameters'
-    gradients in p_dtype"""
-    lib = load()
-    x, rows, inner, so, sr = row_view(x)
-    d = x.shape[-1]
-    dy = dy.contiguous()
-    _dense(dy, rows * d, dev, "dy", x.dtype)
-    dx = _like(x) if need_dx else None
-    dw = torch.empty((d,), device=x.device, dtype=p_dtype) if need_dw else None
-    db = torch.empty((d,), device=x.device, dtype=p_dtype) if need_db else None
-    n = lib.armnet_layer_norm_bwd_ws_bytes(rows, d) if need_dw or need_db else 0
-    ws = torch.empty((n,), device=x.device, dtype=torch.uint8) if n else None
-    mean = st.data_ptr()
-    check(lib.armnet_layer_norm_bwd(rows, inner, so, sr, d, row_type(x, "x"), x.data_ptr(), dy.data_ptr(),
-                                    F32 if p_dtype is None else _ROW_TYPES[p_dtype], _addr(weight), mean, mean + 4 * rows,
-                                    _addr(dx), _addr(dw), _addr(db), _addr(ws), n, _row_stream(dev)))
-    return dx, dw, db
-
-
-def _score_ids(ids, lead, dev, name):
-    """(ids of a row, their type): `ids` [.., n] dense beside rows of the shape `lead`"""
-    if ids is None:
-        return 0, ID_I64
-    if ids.shape[:-1] != lead or not ids.is_contiguous() or ids.get_device() != dev:
-        raise ArmnetNativeError(f"{name}: expected a dense {list(lead) + ['n']} tensor on device {dev}, got {list(ids.shape)} on "
-                                f"{ids.device} (contiguous={ids.is_contiguous()})")
-    return ids.shape[-1], _id_type(ids)
-
-
-@_on_its_device
-def score_logprobs_fwd(dev, X, ids, temperature, top_k, entropy, stats, id_status=None):
-    """armnet_score_logprobs_fwd(X, ids, temperature, top_k, entropy, stats, id_status): ids [.., n_ids] dense or None ->
-    (logp, entropy, top_logp, top_ids, stats), None where not asked for"""
-    lib = load()
-    X, rows, inner, so, sr = row_view(X)
-    c, lead, where, f32 = X.shape[-1], X.shape[:-1], X.device, torch.float32
-    n_ids, id_type = _score_ids(ids, lead, dev, "ids")
-    logp = None if ids is None else torch.empty(ids.shape, device=where, dtype=f32)
-    ent = torch.empty(lead, device=where, dtype=f32) if entropy else None
-    tl = ti = None
-    if top_k:
-        tl = torch.empty(lead + (top_k,), device=where, dtype=f32)
-        ti = torch.empty(lead + (top_k,), device=where, dtype=torch.int64)
-    st = torch.empty((rows, 2), device=where, dtype=f32) if stats else None
-    n = lib.armnet_score_ws_bytes(rows, c, top_k)
-    ws = torch.empty((n,), device=where, dtype=torch.uint8) if n > 0 else None
-    if rows:
-        check(lib.armnet_score_logprobs_fwd(rows, inner, so, sr, c, row_type(X, "X"), X.data_ptr(), temperature, n_ids, _addr(ids),
-                                            id_type, top_k, _addr(logp), _addr(ent), _addr(tl), _addr(ti), _addr(st), _addr(ws),
-                                            n, _addr(id_status), _row_stream(dev)))
-    return logp, ent, tl, ti, st
-
-
-@_on_its_device
-def score_logprobs_bwd(dev, X, ids, temperature, stats, entropy, g_logp, g_entropy):
-    """armnet_score_logprobs_bwd(X, ids, temperature, stats, entropy, g_logp, g_entropy): the gradient of X (dense) from those of
-    logp and entropy (either may be None)"""
-    X, rows, inner, so, sr = row_view(X)
-    n_ids, id_type = _score_ids(ids, X.shape[:-1], dev, "ids")
-    _dense(g_logp, rows * n_ids, dev, "the gradient of logp", torch.float32)
-    _dense(g_entropy, rows, dev, "the gradient of entropy", torch.float32)
-    dx = _like(X)
-    if rows:
-        check(load().armnet_score_logprobs_bwd(rows, inner, so, sr, X.shape[-1], row_type(X, "X"), X.data_ptr(), temperature, n_ids,
-                                               _addr(ids), id_type, stats.data_ptr(), _addr(entropy), _addr(g_logp),
-                                               _addr(g_entropy), dx.data_ptr(), _row_stream(dev)))
-    return dx
-
-
-@_on_its_device
-def distill_fwd(dev, X, ids, teacher, temperature, stats, id_status=None):
-    """armnet_distill_fwd(X, ids, teacher, temperature, stats, id_status): (loss per row, stats for the backward or None); ids and
-    teacher [.., k] dense"""
-    lib = load()
-    X, rows, inner, so, sr = row_view(X)
-    c, lead = X.shape[-1], X.shape[:-1]
-    k, id_type = _score_ids(ids, lead, dev, "top_ids")
-    _dense(teacher, rows * k, dev, "top_scores", teacher.dtype)
-    loss = torch.empty(lead, device=X.device, dtype=torch.float32)
-    st = torch.empty((rows, 4), device=X.device, dtype=torch.float32) if stats else None
-    n = lib.armnet_score_ws_bytes(rows, c, 0)
-    ws = torch.empty((n,), device=X.device, dtype=torch.uint8) if n > 0 else None
-    if rows:
-        check(lib.armnet_distill_fwd(rows, inner, so, sr, c, row_type(X, "X"), X.data_ptr(), temperature, k, ids.data_ptr(), id_type,
-                                     row_type(teacher, "top_scores"), teacher.data_ptr(), loss.data_ptr(), _addr(st), _addr(ws), n,
-                                     _addr(id_status), _row_stream(dev)))
-    return loss, st
-
-
-@_on_its_device
-def distill_bwd(dev, X, ids, teacher, temperature, stats, g_loss):
-    """armnet_distill_bwd(X, ids, teacher, temperature, stats, g_loss): the gradient of X (dense) from that of the rows' losses"""
-    X, rows, inner, so, sr = row_view(X)
-    k, id_type = _score_ids(ids, X.shape[:-1], dev, "top_ids")
-    _dense(g_loss, rows, dev, "the gradient of the loss", torch.float32)
-    dx = _like(X)
-    if rows:
-        check(load().armnet_distill_bwd(rows, inner, so, sr, X.shape[-1], row_type(X, "X"), X.data_ptr(), temperature, k,
-                                        ids.data_ptr(), id_type, row_type(teacher, "top_scores"), teacher.data_ptr(),
-                                        stats.data_ptr(), g_loss.data_ptr(), dx.data_ptr(), _row_stream(dev)))
-    return dx
+def rows():
+    """The row operators' calls and autograd nodes (csrc/row_autograd.cpp, built by the same make), bound to the entries of the
+    library that load() loads."""
+    global _rows
+    if _rows is None:
+        lib = load()
+        if not os.path.exists(ROWS_PATH):
+            raise ArmnetNativeError(f"{ROWS_PATH} is missing: run `python -c 'import __graft_entry__ as g; g.build()'` "
+                                    f"(or `make -C {CSRC}`). There is no CPU fallback for this path.")
+        spec = importlib.util.spec_from_file_location("_armnet_rows", ROWS_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in EXPORTS}, ArmnetNativeError)
+        _rows = mod
+    return _rows

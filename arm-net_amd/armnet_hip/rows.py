@@ -18,16 +18,6 @@ from .block import IdStatus, _id_mode
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _once(backward):
-    """A backward that is not itself differentiable.  Most backwards run with gradients off, where there is nothing to mark; they
-    run on the engine's own thread, where every Python step costs several times what it costs the caller."""
-    marked = once_differentiable(backward)
-
-    def call(ctx, *grads):
-        return marked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return call
-
-
 def _place(what, first, *others):
     """True on the device, False on the host; tensors in different places raise"""
     for name, t in others:
@@ -58,23 +48,20 @@ def _poll(status, devices):
 
 # ---- layer norm ----------------------------------------------------------------------------------------------------------
 
-class _LayerNormFn(torch.autograd.Function):
+class _HostLayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, st = native.layer_norm_fwd(x, weight, bias, eps, True) if x.is_cuda else host_ops.layer_norm_fwd(x, weight, bias, eps)
+        y, st = host_ops.layer_norm_fwd(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, st)
         p = weight if weight is not None else bias
         ctx.p_dtype = None if p is None else p.dtype
         return y
 
     @staticmethod
-    @_once
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, st = ctx.saved_tensors
-        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        bwd = native.layer_norm_bwd if x.is_cuda else host_ops.layer_norm_bwd
-        dx, dw, db = bwd(x, dy, weight, st, need_dx, need_dw, need_db, ctx.p_dtype)
-        return dx, dw, db, None
+        return host_ops.layer_norm_bwd(x, dy, weight, st, *ctx.needs_input_grad[:3], ctx.p_dtype) + (None,)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -95,12 +82,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     on_device = _place("x", x, ("weight", weight), ("bias", bias))
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _LayerNormFn.apply(x, weight, bias, float(eps))
     if on_device:
-        return native.layer_norm_fwd(x, weight, bias, float(eps), False)[0]
-    return host_ops.layer_norm_fwd(x, weight, bias, float(eps))[0]
+        return native.rows().layer_norm(x, weight, bias, float(eps))
+    return _HostLayerNormFn.apply(x, weight, bias, float(eps))
 
 
 class HipLayerNorm(nn.LayerNorm):
@@ -127,33 +111,24 @@ class ScoreLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]       # [.., top_k], int64
 
 
-class _ScoreLogprobsFn(torch.autograd.Function):
+class _HostScoreLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, ids, temperature, top_k, entropy, word):
-        if X.is_cuda:
-            logp, ent, tl, ti, st = native.score_logprobs_fwd(X, ids, temperature, top_k, entropy, True, word)
-        else:
-            logp, ent, tl, ti = host_ops.score_logprobs_fwd(X, ids, temperature, top_k, entropy)
-            st = None
-        ctx.save_for_backward(X, ids, st, ent)
+    def forward(ctx, X, ids, temperature, top_k, entropy):
+        logp, ent, tl, ti = host_ops.score_logprobs_fwd(X, ids, temperature, top_k, entropy)
+        ctx.save_for_backward(X, ids, ent)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*(t for t in (tl, ti) if t is not None))
         return logp, ent, tl, ti
 
     @staticmethod
-    @_once
+    @once_differentiable
     def backward(ctx, g_logp, g_entropy, _tl, _ti):
-        X, ids, st, ent = ctx.saved_tensors
-        if g_logp is None and g_entropy is None:
-            return (None,) * 6
-        g_logp = None if g_logp is None else g_logp.contiguous()
-        g_entropy = None if g_entropy is None else g_entropy.contiguous()
-        if X.is_cuda:
-            dx = native.score_logprobs_bwd(X, ids, ctx.temperature, st, ent, g_logp, g_entropy)
-        else:
+        X, ids, ent = ctx.saved_tensors
+        dx = None
+        if g_logp is not None or g_entropy is not None:
             dx = host_ops.score_logprobs_bwd(X, ids, ctx.temperature, ent, g_logp, g_entropy)
-        return (dx,) + (None,) * 5
+        return (dx,) + (None,) * 4
 
 
 def _row_ids(ids, lead, name):
@@ -195,12 +170,10 @@ def score_logprobs(X, ids=None, temperature=1.0, top_k=0, entropy=False, check_i
         word = None if status is None else status.word()
     elif ids is not None:
         host_ops._check_ids(ids, X.shape[-1], check_ids)
-    if torch.is_grad_enabled() and X.requires_grad:
-        out = _ScoreLogprobsFn.apply(X, ids, t, top_k, bool(entropy), word)
-    elif on_device:
-        out = native.score_logprobs_fwd(X, ids, t, top_k, bool(entropy), False, word)[:4]
+    if on_device:
+        out = native.rows().score_logprobs(X, ids, t, top_k, bool(entropy), word)
     else:
-        out = host_ops.score_logprobs_fwd(X, ids, t, top_k, bool(entropy))
+        out = _HostScoreLogprobsFn.apply(X, ids, t, top_k, bool(entropy))
     if sync:
         status.poll(X.device)
     return ScoreLogprobs(out[0].squeeze(-1) if one else out[0], *out[1:])
@@ -227,27 +200,18 @@ class HipScoreLogprobs(nn.Module):
 
 # ---- distillation --------------------------------------------------------------------------------------------------------
 
-class _DistillFn(torch.autograd.Function):
+class _HostDistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, X, ids, teacher, temperature, word):
-        if X.is_cuda:
-            loss, st = native.distill_fwd(X, ids, teacher, temperature, True, word)
-        else:
-            loss, st = host_ops.distill_fwd(X, ids, teacher, temperature), None
-        ctx.save_for_backward(X, ids, teacher, st)
+    def forward(ctx, X, ids, teacher, temperature):
+        ctx.save_for_backward(X, ids, teacher)
         ctx.temperature = temperature
-        return loss
+        return host_ops.distill_fwd(X, ids, teacher, temperature)
 
     @staticmethod
-    @_once
+    @once_differentiable
     def backward(ctx, g):
-        X, ids, teacher, st = ctx.saved_tensors
-        g = g.contiguous()
-        if X.is_cuda:
-            dx = native.distill_bwd(X, ids, teacher, ctx.temperature, st, g)
-        else:
-            dx = host_ops.distill_bwd(X, ids, teacher, ctx.temperature, g)
-        return dx, None, None, None, None
+        X, ids, teacher = ctx.saved_tensors
+        return host_ops.distill_bwd(X, ids, teacher, ctx.temperature, g), None, None, None
 
 
 def distill_loss(X, top_ids, top_scores, temperature=1.0, check_ids=True, status=None):
@@ -279,12 +243,10 @@ def distill_loss(X, top_ids, top_scores, temperature=1.0, check_ids=True, status
         word = None if status is None else status.word()
     else:
         host_ops._check_ids(ids, X.shape[-1], check_ids)
-    if torch.is_grad_enabled() and X.requires_grad:
-        loss = _DistillFn.apply(X, ids, teacher, t, word)
-    elif on_device:
-        loss = native.distill_fwd(X, ids, teacher, t, False, word)[0]
+    if on_device:
+        loss = native.rows().distill_loss(X, ids, teacher, t, word)
     else:
-        loss = host_ops.distill_fwd(X, ids, teacher, t)
+        loss = _HostDistillFn.apply(X, ids, teacher, t)
     if sync:
         status.poll(X.device)
     return loss

@@ -3,6 +3,7 @@
 U = 2^-24 is half a step of fp32.  A sum of n terms in any order is off by at most (its longest chain of additions) * U * the
 sum of the terms' magnitudes; `chain(n)` bounds that length for the kernels: a row's sum runs over at least 64 threads (a
 wave), then over a tree; a product, a subtraction or an exponential adds a few U."""
+import ctypes
 import math
 
 import torch
@@ -159,3 +160,21 @@ def close(got, ref, tol):
         over = (got - ref).abs()[fine] - tol[fine]
         i = int(over.argmax())
         assert float(over.max()) <= 0, f"off by {float((got - ref).abs()[fine][i]):.3g}, {float(tol[fine][i]):.3g} allowed, at {float(ref[fine][i]):.6g}"
+
+
+def declare_row_calls(lib):
+    """argument types of the row operators' C entries, so that plain numbers and addresses can be passed"""
+    i, l, f, p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+    view = [l, l, l, l, l, i, p]                        # rows, inner, outer_stride, row_stride, last dimension, type, x
+    ids = [f, l, p, i]                                  # temperature, ids of a row, ids, their type
+    for name, args, res in (
+            ("armnet_layer_norm_fwd", view + [i, p, p, f, p, p, p, p], i),
+            ("armnet_layer_norm_bwd_ws_bytes", [l, l], l),
+            ("armnet_layer_norm_bwd", view + [p, i, p, p, p, p, p, p, p, l, p], i),
+            ("armnet_score_ws_bytes", [l, l, i], l),
+            ("armnet_score_logprobs_fwd", view + ids + [i, p, p, p, p, p, p, l, p, p], i),
+            ("armnet_score_logprobs_bwd", view + ids + [p, p, p, p, p, p], i),
+            ("armnet_distill_fwd", view + ids + [i, p, p, p, p, l, p, p], i),
+            ("armnet_distill_bwd", view + ids + [i, p, p, p, p, p], i)):
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, res

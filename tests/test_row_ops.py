@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from armnet_hip import HipDistillLoss, HipLayerNorm, HipScoreLogprobs, distill_loss, layer_norm, native, score_logprobs
-from row_util import close, distill_ref, logp_tol, norm_tol, scores_ref
+from row_util import close, declare_row_calls, distill_ref, logp_tol, norm_tol, scores_ref
 
 Error = native.ArmnetNativeError
 INF = math.inf
@@ -190,6 +190,7 @@ def test_c_entries_check_their_arguments():
     if torch.cuda.is_available():
         pytest.skip("made-up addresses: only where nothing can be launched")
     lib = native.load()
+    declare_row_calls(lib)
     bad, unsup, ok = native.ERR_BAD_ARG, native.ERR_UNSUPPORTED, native.OK
     P = 1 << 20                                                  # an address that is never used: no call below launches
     view = lambda rows=4, d=8, ty=0, x=P: (rows, 0, 0, d, d, ty, x)      # noqa: E731
@@ -241,7 +242,7 @@ def test_row_views_need_no_copy():
     base = torch.arange(2 * 3 * 4 * 6.).view(2, 3, 4, 6)
 
     def rows_of(x):
-        y, rows, inner, so, sr = native.row_view(x)
+        y, rows, inner, so, sr = native.rows().rows_of(x)
         d = y.shape[-1]
         st = y.untyped_storage()
         flat = torch.empty(0, dtype=y.dtype).set_(st)
