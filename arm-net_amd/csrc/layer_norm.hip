@@ -220,11 +220,12 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
         mean = a.mean[q];
         rstd = a.rstd[q];
     };
-    int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+    // the forward's last rows first: some are still in the last-level cache
+    int64_t r = (rounds - 1) * step + (int64_t)blockIdx.x * GROUPS + group;
     load(r);
     float w[NV][V], dw[NV][V] = {}, db[NV][V] = {};
     cols.param(a.weight, a.w_type, 1.f, w);
-    for (int64_t k = 0; k < rounds; ++k, r += step) {
+    for (int64_t k = 0; k < rounds; ++k, r -= step) {
         const bool in = r < a.rows;
         const float rs = rstd;
         float h[NV][V], g[NV][V];
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
             for (int e = 0; e < V; ++e) h[i][e] = (h[i][e] - mean) * rs;
             cols.own(i, g[i]);                         // 0 in g makes 0 of everything below
         }
-        if (k + 1 < rounds) load(r + step);
+        if (k + 1 < rounds) load(r - step);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -544,7 +545,7 @@ static NormShape norm_fwd_shape(int64_t np) {
     if (np <= 128) return {WAVE, 1, 2, LN_TPB};
     if (np <= 256) return {WAVE, 4, 1, LN_TPB};
     if (np <= 512) return {WAVE, 4, 2, LN_TPB};        // (16384 x 4096 bf16: 46 us; eight waves with one piece a lane 55)
-    if (np <= 1024) return {WAVE, 16, 1, 1024};
+    if (np <= 1024) return {WAVE, 8, 2, 512};          // (8000 x 8192 bf16: 43 us; sixteen waves with one piece a lane 65)
     if (np <= 2048) return {WAVE, 16, 2, 1024};
     return {WAVE, 16, 4, 1024};
 }
@@ -598,7 +599,7 @@ static bool launch_norm_fwd(const NormArgs& a, hipStream_t st) {
     if (try_norm_fwd<T, 1, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 2, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 4, 1, 1, 256>(s, a, st) ||
         try_norm_fwd<T, 8, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 16, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 32, 1, 1, 256>(s, a, st) ||
         try_norm_fwd<T, 64, 1, 1, 256>(s, a, st) || try_norm_fwd<T, 64, 1, 2, 256>(s, a, st) || try_norm_fwd<T, 64, 4, 1, 256>(s, a, st) ||
-        try_norm_fwd<T, 64, 4, 2, 256>(s, a, st) || try_norm_fwd<T, 64, 16, 1, 1024>(s, a, st) ||
+        try_norm_fwd<T, 64, 4, 2, 256>(s, a, st) || try_norm_fwd<T, 64, 8, 2, 512>(s, a, st) ||
         try_norm_fwd<T, 64, 16, 2, 1024>(s, a, st))
         return true;
     if constexpr (sizeof(T) == 4) return try_norm_fwd<T, 64, 16, 4, 1024>(s, a, st);

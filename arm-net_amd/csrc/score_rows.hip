@@ -244,17 +244,18 @@ __device__ int best_scores(const T* x, int n, uint32_t id0, const Peak& pk, int 
     if constexpr (NW > 1) maxima[tid] = m;
     if (tid == 0) ts.n = ts.threads = 0;
     group_sync<NW>();
+    constexpr int SPARE = sizeof(T) == 2 ? 13 : 0;                // of a 16-bit score's key the lower 13 bits say nothing
     if (wave == 0) {                     // between lo (reached by >= top threads) and hi (by fewer), until lo is close
         uint32_t k[NW];
         float mn = m, mx = m;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const float v = NW > 1 ? maxima[i * WAVE + lane] : m;
-            k[i] = value_key(v);
+            k[i] = value_key(v) >> SPARE;
             mn = fminf(mn, v);
             mx = fmaxf(mx, v);
         }
-        uint32_t lo = value_key(-wave_max(-mn)), hi = value_key(wave_max(mx)) + 1;
+        uint32_t lo = value_key(-wave_max(-mn)) >> SPARE, hi = (value_key(wave_max(mx)) >> SPARE) + 1;
         int reach = NT;
         uint32_t mid = lo + 1;           // first: are there `top` threads at all above the least (those without a score)?
         while (hi - lo > 1 && reach > top + 8) {
@@ -264,7 +265,8 @@ __device__ int best_scores(const T* x, int n, uint32_t id0, const Peak& pk, int 
             if (c >= top) { lo = mid; reach = c; } else hi = mid;
             mid = lo + (hi - lo) / 2;
         }
-        if (lane == 0) ts.cut = lo;
+        lo <<= SPARE;                    // a negative score's key ends in ones
+        if (lane == 0) ts.cut = lo & 0x80000000u ? lo : lo | ((1u << SPARE) - 1);
     }
     group_sync<NW>();
     const uint32_t cut = ts.cut;
@@ -688,6 +690,23 @@ struct ShortKey<bf16_t> : ShortKey16 {};
 template <>
 struct ShortKey<f16_t> : ShortKey16 {};
 
+// the largest key of aligned groups of LPR lanes, in each of them
+template <int LPR, typename K>
+__device__ __forceinline__ K lanes_max_key(K k) {
+    auto step = [&](auto exchange) {
+        K o;
+        if constexpr (sizeof(K) == 4) o = exchange((uint32_t)k);
+        else o = ((K)exchange((uint32_t)(k >> 32)) << 32) | exchange((uint32_t)k);
+        k = o > k ? o : k;
+    };
+    if constexpr (LPR >= 2) step([](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xb1, 0xf, 0xf, false); });
+    if constexpr (LPR >= 4) step([](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4e, 0xf, 0xf, false); });
+    if constexpr (LPR >= 8) step([](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false); });
+    if constexpr (LPR >= 16) step([](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xf, 0xf, false); });
+    static_assert(LPR <= 16, "within a row of 16 lanes");
+    return k;
+}
+
 template <typename T, int LPR, int P, bool ENT, bool TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
     typedef ShortKey<T> Key;
@@ -771,41 +790,56 @@ __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
                 }
             }
         }
-        if constexpr (TOP) {                           // a score's rank: how many of the row are better
-            typename Key::type* mine = keys + slot * W;
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (e >= row.lo[i]) {
-                        const uint32_t col = row.off[i] + e;
-                        mine[col] = Key::of(row.v[i][e], col);
-                    }
-            group_sync<1>();
+        if constexpr (TOP) {
+            const bool nan = s.S != s.S;
             typename Key::type key[P][V];
-            int rank[P][V] = {};
+            auto write = [&](int i, int e, int rank) {
+                const bool live = !nan && Key::live(key[i][e]);
+                a.top_ids[r * a.top + rank] = live ? row.off[i] + e : -1;
+                a.top_logp[r * a.top + rank] = nan ? NAN : live ? (row.v[i][e] - s.m) * a.rt - LN2 * l2 : -INFINITY;
+            };
 #pragma unroll
             for (int i = 0; i < P; ++i)
 #pragma unroll
-                for (int e = 0; e < V; ++e) key[i][e] = e >= row.lo[i] ? mine[row.off[i] + e] : 0;
-            for (int j = 0; j < a.c; ++j) {
-                const typename Key::type other = mine[j];
+                for (int e = 0; e < V; ++e) key[i][e] = e >= row.lo[i] ? Key::of(row.v[i][e], row.off[i] + e) : 0;
+            if (3 * a.top <= a.c) {                    // few: the largest key below the last one, again and again
+                typename Key::type last = ~(typename Key::type)0;
+                for (int k = 0; k < a.top; ++k) {
+                    typename Key::type most = 0;
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) most = key[i][e] < last && key[i][e] > most ? key[i][e] : most;
+                    last = lanes_max_key<LPR>(most);
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (in && key[i][e] == last) write(i, e, k);
+                }
+            } else {                                   // many: a score's rank is how many of the row are better
+                typename Key::type* mine = keys + slot * W;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) rank[i][e] += other > key[i][e] ? 1 : 0;
+                    for (int e = 0; e < V; ++e)
+                        if (e >= row.lo[i]) mine[row.off[i] + e] = key[i][e];
+                group_sync<1>();
+                int rank[P][V] = {};
+                for (int j = 0; j < a.c; ++j) {
+                    const typename Key::type other = mine[j];
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) rank[i][e] += other > key[i][e] ? 1 : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (in && e >= row.lo[i] && rank[i][e] < a.top) write(i, e, rank[i][e]);
+                group_sync<1>();
             }
-            const bool nan = s.S != s.S;
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (in && e >= row.lo[i] && rank[i][e] < a.top) {
-                        const bool live = !nan && Key::live(key[i][e]);
-                        a.top_ids[r * a.top + rank[i][e]] = live ? row.off[i] + e : -1;
-                        a.top_logp[r * a.top + rank[i][e]] = nan ? NAN : live ? (row.v[i][e] - s.m) * a.rt - LN2 * l2 : -INFINITY;
-                    }
-            group_sync<1>();
         }
     }
 }
@@ -999,8 +1033,9 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
     float* s_g = (float*)(s_id + n16);
     const int64_t units = a.rows * a.splits;
     for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
-        const int64_t r = a.splits == 1 ? unit : unit / a.splits;
-        const int from = (int)((unit - r * a.splits) * a.per);
+        const int64_t back = units - 1 - unit;          // the forward's last rows first: some are still in the last-level cache
+        const int64_t r = a.splits == 1 ? back : back / a.splits;
+        const int from = (int)((back - r * a.splits) * a.per);
         const int n = (int)(a.per < a.c - from ? a.per : a.c - from);
         const int nvec = n / V, rem = n - nvec * V;
         const T* x = row_ptr<T>(a.x, r) + from;
