@@ -184,11 +184,12 @@ def score_logprobs_bwd(X, ids, temperature, entropy, g_logp, g_entropy):
     if g_logp is not None:
         ok = (ids >= 0) & (ids < x.shape[-1]) & live
         g = torch.where(ok, g_logp.to(p.dtype), torch.zeros((), dtype=p.dtype))
-        dz = -p * g.sum(-1, keepdim=True)
+        dz = torch.where(ok.any(-1, keepdim=True), -p * g.sum(-1, keepdim=True), torch.zeros_like(p))    # padding: 0, whatever it holds
         dz = dz.scatter_add(-1, ids.long().clamp(0, x.shape[-1] - 1), g)
     if g_entropy is not None:
         t = torch.where(p == 0, torch.zeros_like(p), p * (lp + entropy.to(p.dtype).unsqueeze(-1)))
-        dz = dz - g_entropy.to(p.dtype).unsqueeze(-1) * t
+        gh = g_entropy.to(p.dtype).unsqueeze(-1)
+        dz = dz - torch.where(gh == 0, torch.zeros_like(t), gh * t)
     return (dz / temperature).to(X.dtype)
 
 
@@ -215,6 +216,6 @@ def distill_bwd(X, ids, teacher, temperature, g_loss):
     _, q = _teacher(ids, teacher, temperature, x.dtype)
     told = q.sum(-1, keepdim=True)
     told = torch.where(told > 0, torch.ones_like(told), told)
-    d = (p * told).scatter_add(-1, ids.long().clamp(0, c - 1),
+    d = torch.where(told == 0, torch.zeros_like(p), p * told).scatter_add(-1, ids.long().clamp(0, c - 1),
                                torch.where((ids >= 0) & (ids < c) & live, -q, torch.zeros_like(q)))
     return (d * (g_loss.to(x.dtype) * temperature).unsqueeze(-1)).to(X.dtype)

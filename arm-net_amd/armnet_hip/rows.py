@@ -154,7 +154,8 @@ def score_logprobs(X, ids=None, temperature=1.0, top_k=0, entropy=False, check_i
     entropy   -sum p log p per row
 
     A score of -inf is masked: it is no alternative (slots past the last unmasked score: -inf and -1).  A row of nothing but
-    -inf: log p -inf, entropy 0, gradient 0.  A row with a NaN or +inf: NaN, alternatives -1.  Differentiable in X through logp
+    -inf: log p -inf, entropy 0, gradient 0.  A row with a NaN or +inf: NaN, alternatives -1.  A row of empty slots (padding) whose
+    entropy has no gradient or 0: gradient 0, whatever it holds.  Differentiable in X through logp
     and entropy (not through top_logp: pass top_ids as ids for that)."""
     _float_rows(X, "X")
     t = _temperature(temperature)
@@ -222,7 +223,7 @@ def distill_loss(X, top_ids, top_scores, temperature=1.0, check_ids=True, status
 
     top_ids, top_scores: [.., k], k <= 1024; a negative id is an empty slot, an id >= C an IndexError (check_ids / status as for
     score_logprobs()).  score_logprobs(teacher_scores, top_k=k) gives both: its top_logp are the teacher's scores up to a
-    constant that q does not see (at temperature 1).  A row without a teacher: loss and gradient 0.  An id that is listed
+    constant that q does not see (at temperature 1).  A row without a teacher: loss and gradient 0, whatever X holds there.  An id that is listed
     twice counts twice.  A student's row of nothing but -inf: loss +inf, gradient 0.  Differentiable in X; the teacher is a
     constant (top_scores that require a gradient raise)."""
     _float_rows(X, "X")

@@ -8,9 +8,10 @@
 //   dx_j = g T (p_j - sum_k q_k 1(id_k = j))
 //
 // Sums are held in base 2 (z2 = z log2 e, exponentials by the hardware's exp2) and everything in fp32; log p is
-// (x - m) / T - ln2 log2 S, as far as fp32 reaches.  Gradients are rounded once, to x's type.  m starts at the lowest finite number instead of -inf: a masked score (-inf) then has z = -inf and e^z = 0
-// without a special case, a row of the lowest number has p = 1/C, and S = 0 says that nothing in the row is above -inf.
-// (m, log2 S) go from the forward to the backward as two numbers: their sum would lose what m's magnitude takes.
+// (x - m) / T - ln2 log2 S, as far as fp32 reaches.  Gradients are rounded once, to x's type.  m starts at the lowest finite
+// number instead of -inf: a masked score (-inf) then has z = -inf and e^z = 0 without a special case, a row of the lowest number
+// has p = 1/C, and S = 0 says that nothing in the row is above -inf.  (m, log2 S) go from the forward to the backward as two
+// numbers: their sum would lose what m's magnitude takes.
 #include "row_common.h"
 
 namespace armnet {
@@ -182,21 +183,6 @@ struct TopScratch {
     int count[NW];
     uint8_t who[NW * WAVE];
 };
-
-// how many threads of the group say yes, in every thread
-template <int NW>
-__device__ __forceinline__ int group_count(bool yes, int* count) {
-    int n = __popcll(__ballot(yes));
-    if constexpr (NW > 1) {
-        __syncthreads();
-        if ((threadIdx.x & (WAVE - 1)) == 0) count[threadIdx.x / WAVE] = n;
-        __syncthreads();
-        n = 0;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) n += count[i];
-    }
-    return n;
-}
 
 template <int NW>
 __device__ __forceinline__ void push(TopScratch<NW>& ts, float v, uint32_t id) {
@@ -863,6 +849,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
         for (int i = tid; i < a.c; i += LPR) mine[i] = 0.f;
         group_sync<1>();
         float sum = 0.f;
+        float used = 0.f;
         for (int k0 = 0; k0 < a.n_ids; k0 += LPR) {
             int at = -1;
             float g = 0.f;
@@ -870,6 +857,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
                 const int64_t k = r * a.n_ids + k0 + tid, id = load_id(a.ids, a.id_type, k);
                 if (id >= 0 && id < a.c && !none) {
                     at = (int)id;
+                    used = 1.f;
                     if (DISTILL) g = exp2_raw((load_any(a.teacher, a.t_type, k) - mt) * a.c2 - lt);
                     else if (a.g_logp) g = a.g_logp[k];
                     sum += g;
@@ -885,7 +873,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
         float A, B = 0.f, H2 = 0.f, u;
         if (DISTILL) {
             u = -a.g_logp[r] * a.t;
-            A = lt == INFINITY ? 0.f : -u + (lt - lt);
+            A = -u + (lt - lt);
         } else {
             A = -lanes_sum<LPR>(sum) * a.rt;
             u = a.rt;
@@ -894,6 +882,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
                 H2 = a.entropy[r] / LN2;
             }
         }
+        const bool dead = DISTILL ? lt == INFINITY : lanes_max<LPR>(used) == 0.f && (!ENT || B == 0.f);
         T* dx = (T*)a.dx + r * a.c;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -903,7 +892,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
                 const float lp = fmaf(row.v[i][e] - m, a.c2, -l2);
                 const float p = exp2_raw(lp);
                 const float d = ENT ? p * fmaf(B, fmaxf(lp, Z_FLOOR) + H2, A) : p * A;
-                o[e] = e >= row.lo[i] ? fmaf(mine[row.off[i] + e], u, d) : 0.f;
+                o[e] = e >= row.lo[i] && !dead ? fmaf(mine[row.off[i] + e], u, d) : 0.f;
             }
             if (!in) continue;
             if (row.lo[i] == 0) {
@@ -1054,6 +1043,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         const bool none = l2 == INFINITY;
         group_sync<NW>();                               // the slice before is done with the list
         float sum = 0.f;
+        bool used = false;
         int32_t first = -1;                             // this thread's slot of the list (k = tid), its addend and the row's score
         float first_g = 0.f, first_x = 0.f;
         for (int k0 = 0; k0 < n16; k0 += WAVE) {        // every wave adds up the whole list, each keeps its share of it
@@ -1063,6 +1053,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
             if (k < a.n_ids) {
                 const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
                 const bool in = id >= 0 && id < a.c && !none;
+                used = used || in;
                 if (DISTILL) {
                     if (in) g = exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2 - lt);
                 } else if (in && a.g_logp) {
@@ -1085,7 +1076,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         float A, B = 0.f, H2 = 0.f, u;
         if (DISTILL) {
             u = -a.g_logp[r] * a.t;
-            A = lt == INFINITY ? 0.f : -u + (lt - lt);  // a teacher without a distribution (NaN) has no gradient either
+            A = -u + (lt - lt);                         // a teacher without a distribution (NaN) has no gradient either
         } else {
             A = -wave_sum(sum) * a.rt;
             u = a.rt;
@@ -1094,6 +1085,8 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
                 H2 = a.entropy[r] / LN2;
             }
         }
+        // a row that nothing is asked of has gradient 0, whatever it holds (the padding of a batch)
+        const bool dead = __builtin_amdgcn_readfirstlane(DISTILL ? lt == INFINITY : !__any(used) && (!ENT || B == 0.f));
         auto base = [&](float xv) {
             const float lp = fmaf(xv - m, a.c2, -l2);
             const float p = exp2_raw(lp);
@@ -1106,14 +1099,19 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
                 if (j + tid + i * NT < nvec) {
                     float v[V];
                     Piece<T>::unpack(raw[i], v);
+                    if (dead) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] = base(v[e]);
+                        for (int e = 0; e < V; ++e) v[e] = 0.f;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) v[e] = base(v[e]);
+                    }
                     Piece<T>::store(dx + (int64_t)(j + tid + i * NT) * V, Piece<T>::pack(v));
                 }
             }
         }
-        if (tid < rem) dx[nvec * V + tid] = from_f32<T>(base(to_f32(x[nvec * V + tid])));
-        if (a.n_ids == 0) continue;
+        if (tid < rem) dx[nvec * V + tid] = from_f32<T>(dead ? 0.f : base(to_f32(x[nvec * V + tid])));
+        if (a.n_ids == 0 || dead) continue;
         // the list is complete, and the stores above come before the ones below
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         group_sync<NW>();

@@ -556,7 +556,8 @@ int armnet_layer_norm_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int
  * A score of -inf is masked: it is never an alternative (slots past the last unmasked score hold -inf and -1).  A row of
  * nothing but -inf has log p = -inf and entropy 0; a row with a NaN or +inf has NaN everywhere and no alternatives (-1).
  * An id >= c has log p NaN and sets id_status like everywhere else.  1e-6 <= temperature <= 1e6.
- * workspace: armnet_score_ws_bytes(rows, c, top) bytes, 16-byte aligned, its content unused before and after.
+ * workspace: armnet_score_ws_bytes(rows, c, top) bytes (of the current device), 16-byte aligned, its content unused before and
+ * after.
  */
 int64_t armnet_score_ws_bytes(int64_t rows, int64_t c, int top);
 int armnet_score_logprobs_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
@@ -564,7 +565,8 @@ int armnet_score_logprobs_fwd(int64_t rows, int64_t inner, int64_t outer_stride,
                               float* logp, float* entropy, float* top_logp, int64_t* top_ids, float* stats, void* workspace,
                               int64_t ws_bytes, int32_t* id_status, void* stream);
 /* dx [rows, c] of x's type from g_logp [rows, n_ids] and g_entropy [rows] (either may be NULL; with g_entropy the forward's
- * entropy); the same id in several slots adds up; a row of nothing but -inf has gradient 0 */
+ * entropy); the same id in several slots adds up; a row of nothing but -inf has gradient 0, and so has, whatever it holds, a row
+ * of empty slots whose g_entropy is 0 or not given */
 int armnet_score_logprobs_bwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,
                               const void* x, float temperature, int64_t n_ids, const void* ids, int id_type,
                               const float* stats, const float* entropy, const float* g_logp, const float* g_entropy, void* dx,
@@ -575,7 +577,7 @@ int armnet_score_logprobs_bwd(int64_t rows, int64_t inner, int64_t outer_stride,
  * negative id is an empty slot), p = softmax(x / temperature) over the whole row,
  *   loss [rows] = temperature^2 * sum_k q_k (log q_k - log p[ids_k])
  * teacher [rows, k] of t_type; stats [rows, 4] for the backward, or NULL; workspace as above with top = 0.  A row without a
- * teacher has loss 0 and gradient 0; an id twice in a row's list counts twice.  A row of x with nothing but -inf has loss +inf
+ * teacher has loss 0 and gradient 0, whatever x holds; an id twice in a row's list counts twice.  A row of x with nothing but -inf has loss +inf
  * (where the teacher has weight) and gradient 0.
  */
 int armnet_distill_fwd(int64_t rows, int64_t inner, int64_t outer_stride, int64_t row_stride, int64_t c, int x_type,

@@ -63,7 +63,7 @@ def norm_gradients(x, w, b, dy, dtype, got=None, eps=1e-5):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", NORM_SHAPES + [(700, 16), (3000, 130), (513, 512)])
+@pytest.mark.parametrize("shape", NORM_SHAPES + [(700, 16), (3000, 130), (513, 512), (600, 2050), (300, 9001)])
 def test_layer_norm_gradients(shape, dtype):
     d = shape[-1]
     x, dy = (rnd(*shape) * 0.5 + 1.5).to(dtype), rnd(*shape, seed=3).to(dtype)
@@ -71,6 +71,17 @@ def test_layer_norm_gradients(shape, dtype):
     norm_gradients(x, None, None, dy, dtype)
     norm_gradients(x, rnd(d, seed=1).to(dtype), None, dy, dtype)
     norm_gradients(x, None, rnd(d, seed=1).to(dtype), dy, dtype)
+
+
+@pytest.mark.parametrize("x_type", TYPES)
+@pytest.mark.parametrize("w_type", TYPES)
+@pytest.mark.parametrize("d", [3, 40, 1001, 20001])
+def test_layer_norm_parameters_of_another_type(x_type, w_type, d):
+    x, dy = (rnd(9, d) + 1).to(x_type), rnd(9, d, seed=3).to(x_type)
+    w, b = (1 + 0.1 * rnd(d, seed=1)).to(w_type), (0.1 * rnd(d, seed=2)).to(w_type)
+    y, tol = norm_tol(x, w, b, 1e-5, x_type)
+    close(layer_norm(x.to(DEV), w.to(DEV), b.to(DEV)), y, tol)
+    norm_gradients(x, w, b, dy, x_type)
 
 
 def test_layer_norm_only_the_gradients_that_are_wanted():
@@ -172,6 +183,36 @@ def test_scores(shape, dtype):
     check_scores(x, ids[..., :1].int(), 0.7, min(c, 64), entropy=False)
     check_scores(x, None, 2.0, min(c, 1))
     check_scores(x, ids, 2.0, 0, entropy=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_in_slices(dtype):
+    """more slices than the launch has blocks; the last slice shorter than the alternatives"""
+    x = (rnd(700, 20001) * 3).to(dtype)
+    ids = torch.randint(0, 20001, (700, 2), generator=gen(1))
+    check_scores(x, ids, 1.0, 9)
+    check_scores(x[:3, :8197], ids[:3].clamp(max=8196), 0.9, 64)
+
+
+def test_lists_of_no_ids():
+    x = rnd(4, 30).to(DEV).requires_grad_(True)
+    r = score_logprobs(x, torch.zeros(4, 0, dtype=torch.int64, device=DEV), entropy=True)
+    assert r.logp.shape == (4, 0)
+    g, = torch.autograd.grad((r.logp.sum(), r.entropy.sum()), x)
+    want, = torch.autograd.grad(score_logprobs(x, entropy=True).entropy.sum(), x)
+    assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("c", [30, 3000])
+def test_a_masked_answer_is_a_lesson(c):
+    """alternatives that are not there come as empty slots"""
+    teacher = rnd(5, c)
+    teacher[1, 3:] = -INF
+    teacher[2] = -INF
+    told = score_logprobs(teacher.to(DEV), top_k=8)
+    x = rnd(5, c, seed=1)
+    check_distill(x, told.top_ids.cpu(), told.top_logp.cpu(), 1.5, torch.ones(5), F32)
+    assert distill_loss(x.to(DEV), told.top_ids, told.top_logp)[2] == 0
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -394,6 +435,28 @@ def test_distillation_edges(c, dtype):
     loss = distill_loss(xd, ids.to(DEV), ts.to(DEV), 2.0)
     got, = torch.autograd.grad(loss, xd, g.to(DEV))
     assert loss.isnan().tolist() == [True, True] + [False] * 5 and got[:2].isnan().all() and not got[2:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [9, 40, 700, 5382, 40003])
+@pytest.mark.parametrize("device", ["cpu", DEV])
+def test_padding_has_gradient_zero(c, dtype, device):
+    """rows that nothing is asked of may hold anything"""
+    x = rnd(6, c).to(dtype)
+    x[3] = math.nan
+    x[4, 1] = INF
+    x[5] = torch.finfo(dtype).max
+    ids = torch.tensor([[0, 1], [2, -1], [c - 1, 0], [-1, -1], [-1, -2], [-5, -1]], device=device)
+    ts = rnd(6, 2, seed=1).to(device)
+    xd = x.to(device).requires_grad_(True)
+    up = torch.tensor([1.0, 2.0, 0.5, 0.0, 0.0, 0.0], device=device)
+    r = score_logprobs(xd, ids, entropy=True)
+    for outs, ups in (((r.logp,), (torch.ones(6, 2, device=device),)), ((r.logp, r.entropy), (torch.ones(6, 2, device=device), up))):
+        got, = torch.autograd.grad(outs, xd, ups, retain_graph=True)
+        assert got[3:].eq(0).all() and got[:3].isfinite().all() and got[:3].ne(0).any(-1).all()
+    loss = distill_loss(xd, ids, ts, 1.5)
+    got, = torch.autograd.grad(loss, xd, torch.ones(6, device=device))
+    assert loss[3:].eq(0).all() and got[3:].eq(0).all() and got[:3].isfinite().all() and got[:3].ne(0).any(-1).all()
 
 
 def test_distillation_takes_rows_where_they_are():
