@@ -170,10 +170,10 @@ __device__ __forceinline__ Sums group_sums(Sums s, float c2, float* scratch) {
     return s;
 }
 
-constexpr int SC_UNROLL = 2;             // pieces of 16 bytes in flight a thread
+constexpr int SC_UNROLL = 2;             // pieces of 16 bytes in flight a thread (2048 x 131072 bf16: 96 us; four 106)
 constexpr int SC_BWD_UNROLL = 4;         // ... in the backward, which computes less and has no state to keep
 constexpr int SC_BUF = 512;              // candidates for the alternatives
-constexpr int SC_FEW = 128;              // so few scores are all candidates
+constexpr int SC_FEW = 128;              // so few scores are all candidates (4618 x 73 f32 with 16: 11.2 us; by their bound 13.4)
 
 template <int NW>
 struct TopScratch {
@@ -270,21 +270,17 @@ __device__ int best_scores(const T* x, int n, uint32_t id0, const Peak& pk, int 
             if (pk.at >= 0)
                 for (int u = 0; u < U; ++u)
                     if (pk.at + u * NT < nvec) candidates(pk.at + u * NT);
-        } else if (pieces <= 2 * U) {
-            for (int at = tid; at < nvec; at += NT) candidates(at);
         } else {
             ts.who[atomicAdd(&ts.threads, 1)] = (uint8_t)tid;
         }
     }
-    if (pieces > 2 * U) {                // a wave reads what such a thread owns
-        group_sync<NW>();
-        const int threads = ts.threads;
-        for (int w = wave; w < threads; w += NW)
-            for (int j = lane; j < pieces; j += WAVE) {
-                const int at = j * NT + ts.who[w];
-                if (at < nvec) candidates(at);
-            }
-    }
+    group_sync<NW>();
+    const int threads = ts.threads;      // a wave reads what such a thread owns
+    for (int w = wave; w < threads; w += NW)
+        for (int j = lane; j < pieces; j += WAVE) {
+            const int at = j * NT + ts.who[w];
+            if (at < nvec) candidates(at);
+        }
     if (tid < rem) {
         const float v = to_f32(x[nvec * V + tid]);
         if (v >= cutv) push(ts, v, id0 + nvec * V + tid);
@@ -693,11 +689,12 @@ __device__ __forceinline__ K lanes_max_key(K k) {
     return k;
 }
 
-template <typename T, int LPR, int P, bool ENT, bool TOP, bool DISTILL>
+// TOP: 0 no alternatives, 1 a few, 2 any number of them
+template <typename T, int LPR, int P, bool ENT, int TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
     typedef ShortKey<T> Key;
-    constexpr int V = Piece<T>::N, ROWS = SC_TPB / LPR, W = TOP ? LPR * P * V + 1 : 1;
-    __shared__ typename Key::type keys[TOP ? ROWS * W : 1];
+    constexpr int V = Piece<T>::N, ROWS = SC_TPB / LPR, W = TOP == 2 ? LPR * P * V + 1 : 1;
+    __shared__ typename Key::type keys[TOP == 2 ? ROWS * W : 1];
     const int tid = threadIdx.x & (LPR - 1), slot = threadIdx.x / LPR;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * ROWS) {
         const bool in = r0 + slot < a.rows;            // lanes without a row work on the last one's and write nothing
@@ -788,7 +785,8 @@ __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
             for (int i = 0; i < P; ++i)
 #pragma unroll
                 for (int e = 0; e < V; ++e) key[i][e] = e >= row.lo[i] ? Key::of(row.v[i][e], row.off[i] + e) : 0;
-            if (3 * a.top <= a.c) {                    // few: the largest key below the last one, again and again
+            // few: the largest key below the last one, again and again (131072 x 64 bf16, 8 of 64: 33 us, by ranks 44)
+            if (TOP == 1 || 3 * a.top <= a.c) {
                 typename Key::type last = ~(typename Key::type)0;
                 for (int k = 0; k < a.top; ++k) {
                     typename Key::type most = 0;
@@ -803,7 +801,7 @@ __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
                         for (int e = 0; e < V; ++e)
                             if (in && key[i][e] == last) write(i, e, k);
                 }
-            } else {                                   // many: a score's rank is how many of the row are better
+            } else if constexpr (TOP == 2) {           // many: a score's rank is how many of the row are better
                 typename Key::type* mine = keys + slot * W;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
@@ -912,21 +910,25 @@ static unsigned short_grid(int64_t rows, int lpr) {
     return (unsigned)(blocks < most ? blocks : most);
 }
 
-// Rows this short go several to a wave: 4 lanes with up to four pieces each, or 16.  With alternatives every score of a row is
-// compared with every other: up to 64 of them, 8 or less a lane.
+// Rows of up to 64 pieces go several to a wave: 4 lanes with one piece each, or 16 with up to four (131072 x 64 f32: 12 us, with a
+// wave a row 42; 100000 x 250 f32: 28 and 38).  Alternatives: of up to 64 scores any number; of more by repeated maxima, as long as
+// that beats a wave a row: 20000 x 100 f32 with 5 / 12 / 24 of them 10 / 15 / 24 us, a wave a row 39; 100000 x 250 with 1 / 5 / 10
+// of them bf16 33 / 50 / 73 us, f32 52 / 85 / 122, a wave a row 110 (but of 300 rows 7.8, a wave a row 5.9).
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 static bool launch_short_fwd(const ScoreArgs& a, hipStream_t st) {
     constexpr int V = Piece<T>::N;
     if (DISTILL && a.n_ids > 64) return false;
     if constexpr (TOP) {
-        constexpr int P = sizeof(T) == 4 ? 2 : 1;
-        if (a.c <= 4 * P * V) score_short_fwd_kernel<T, 4, P, ENT, true, false><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
-        else if (a.c <= 64) score_short_fwd_kernel<T, 64 / V, 1, ENT, true, false><<<short_grid(a.rows, 64 / V), SC_TPB, 0, st>>>(a);
+        constexpr int P = sizeof(T) == 4 ? 2 : 1;     // 4 lanes: 32 scores, 16 lanes: 128
+        if (a.c <= 4 * P * V) score_short_fwd_kernel<T, 4, P, ENT, 2, false><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 64) score_short_fwd_kernel<T, 64 / V, 1, ENT, 2, false><<<short_grid(a.rows, 64 / V), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 128 && a.top <= 40) score_short_fwd_kernel<T, 16, P, ENT, 1, false><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 256 && a.top <= 8 && a.rows >= 4096) score_short_fwd_kernel<T, 16, 2 * P, ENT, 1, false><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
         else return false;
     } else {
-        if (a.c <= 4 * V) score_short_fwd_kernel<T, 4, 1, ENT, false, DISTILL><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
-        else if (a.c <= 16 * V) score_short_fwd_kernel<T, 16, 1, ENT, false, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
-        else if (a.c <= 64 * V) score_short_fwd_kernel<T, 16, 4, ENT, false, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
+        if (a.c <= 4 * V) score_short_fwd_kernel<T, 4, 1, ENT, 0, DISTILL><<<short_grid(a.rows, 4), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 16 * V) score_short_fwd_kernel<T, 16, 1, ENT, 0, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
+        else if (a.c <= 64 * V) score_short_fwd_kernel<T, 16, 4, ENT, 0, DISTILL><<<short_grid(a.rows, 16), SC_TPB, 0, st>>>(a);
         else return false;
     }
     return true;

@@ -314,7 +314,7 @@ def test_score_gradients_masks(c, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,c", [(70001, 2), (40007, 10), (20001, 33), (9001, 64), (5003, 250), (4999, 2050), (4100, 5382)])
+@pytest.mark.parametrize("n,c", [(70001, 2), (40007, 10), (20001, 33), (9001, 64), (6001, 100), (5003, 250), (4999, 2050), (4100, 5382)])
 def test_many_rows(n, c, dtype):
     """several rows a wave, a wave a row, more rows than the launch has waves"""
     x = (rnd(n, c) * 2).to(dtype)
