@@ -146,7 +146,10 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
     return v;
 }
 
-// One row group: LPR lanes (NW = 1) or NW waves.  A block holds TPB / (LPR or NW * 64) of them.
+// One row group: LPR lanes (NW = 1) or NW waves.  A block holds TPB / (LPR or NW * 64) of them and goes on to further rows; the next
+// row is asked for as soon as this one is unpacked, into the same registers.  Bound by memory: 65536 x 512 f32 in 51 us (5.3 TB/s),
+// 16384 x 4096 bf16 in 47 (5.7), 8000 x 8192 bf16 in 43 (6.1; a large copy moves 5.2); rows whose length is no multiple of 16 bytes
+// are slower (10007 x 2049 f16, whose last piece keeps another half of the block busy: 22 us, 3.7 TB/s).
 template <typename T, int LPR, int NW, int NV, int TPB>
 __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
     constexpr int V = Piece<T>::N, NT = LPR < WAVE ? LPR : NW * WAVE, GROUPS = TPB / NT;
@@ -199,13 +202,40 @@ __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
     }
 }
 
-// dx of a row, and the block's share of dw and db: in registers over its rows, then over its groups through LDS
-template <typename T, int LPR, int NW, int NV, int TPB>
+// A lane's own values between the rows, in LDS instead of registers: [NV][V] floats as 16-byte cells, nobody else's.
+template <int NV, int V, int TPB>
+struct LaneCells {
+    static constexpr int N = NV * V / 4;
+    static __device__ __forceinline__ void put(float4 (*cells)[TPB], int i, const float (&f)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) cells[(i * V + e) / 4][threadIdx.x] = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+    }
+    static __device__ __forceinline__ void put(float4 (*cells)[TPB], const float (&f)[NV][V]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) put(cells, i, f[i]);
+    }
+    static __device__ __forceinline__ void get(const float4 (*cells)[TPB], int i, float (&f)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const float4 q = cells[(i * V + e) / 4][threadIdx.x];
+            f[e] = q.x, f[e + 1] = q.y, f[e + 2] = q.z, f[e + 3] = q.w;
+        }
+    }
+};
+
+// dx of a row, and the block's share of dw and db: in registers over its rows, then over its groups through LDS.  x and dy are read
+// once for all three.  Bound by memory: with the sum over the blocks 65536 x 512 f32 in 82 us (4.9 TB/s), 16384 x 4096 bf16 in 80 (5.0);
+// of more than 8192 values less (1500 x 16384 f32 in 76, 3.9 TB/s): one row a CU is in work, one on its way.  A few hundred long rows
+// cost what the blocks' shares cost (1000 x 10000 bf16: 36 us, of which the rows 12).
+// KEEP: what waits in LDS between the rows instead of in registers: 0 nothing, 1 the weights, 2 the sums for dw too.
+template <typename T, int LPR, int NW, int NV, int TPB, int KEEP>
 __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
     constexpr int V = Piece<T>::N, NT = LPR < WAVE ? LPR : NW * WAVE, GROUPS = TPB / NT;
     __shared__ float scratch[2][2][TPB / WAVE];
     constexpr int SHARES = LPR < WAVE ? TPB / WAVE : GROUPS;     // short rows: a wave's groups meet in registers
     __shared__ float sums[2][SHARES > 1 ? NV * NT * V : 1];
+    using Cells = LaneCells<NV, V, TPB>;
+    __shared__ float4 w_cells[KEEP >= 1 ? Cells::N : 1][KEEP >= 1 ? TPB : 1], dw_cells[KEEP >= 2 ? Cells::N : 1][KEEP >= 2 ? TPB : 1];
     const int group = threadIdx.x / NT, tid = threadIdx.x & (NT - 1);
     const Columns<T, NT, NV> cols(a.d, tid);
     const float rd = 1.f / (float)a.d;
@@ -225,6 +255,8 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
     load(r);
     float w[NV][V], dw[NV][V] = {}, db[NV][V] = {};
     cols.param(a.weight, a.w_type, 1.f, w);
+    if constexpr (KEEP >= 1) Cells::put(w_cells, w);
+    if constexpr (KEEP >= 2) Cells::put(dw_cells, dw);
     for (int64_t k = 0; k < rounds; ++k, r -= step) {
         const bool in = r < a.rows;
         const float rs = rstd;
@@ -240,7 +272,9 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
         }
         if (k + 1 < rounds) load(r - step);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (KEEP >= 1) Cells::get(w_cells, i, w[i]);
+            if constexpr (KEEP >= 2) Cells::get(dw_cells, i, dw[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 if (in) {
@@ -251,6 +285,8 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
                 s1 += g[i][e];
                 s2 = fmaf(g[i][e], h[i][e], s2);
             }
+            if constexpr (KEEP >= 2) Cells::put(dw_cells, i, dw[i]);
+        }
         if (a.out) {
             float m1, m2;
             if constexpr (NW == 1) {
@@ -287,6 +323,9 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
         }
     }
     if (!a.params) return;
+    if constexpr (KEEP >= 2)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) Cells::get(dw_cells, i, dw[i]);
     int share = group;
     if constexpr (LPR < WAVE) {
 #pragma unroll
@@ -362,6 +401,9 @@ __global__ void __launch_bounds__(LN_SUM_WAVES * WAVE) norm_param_kernel(const f
 }
 
 // ---- rows longer than LN_MAX_D: a block a row, read again for each step ---------------------------------------------------
+//
+// Bound by reading a row three times (of which the caches serve a part): 1000 x 20000 f32 forward in 45 us, 3.6 TB/s of what it cannot
+// do without; backward, with the parameters' gradients in a pass of their own, 105 us, 2.3 TB/s.
 
 constexpr int LN_LONG_TPB = 1024, LN_LONG_NW = LN_LONG_TPB / WAVE;
 
@@ -589,7 +631,10 @@ static bool try_norm_fwd(const NormShape& s, const NormArgs& a, hipStream_t st) 
 template <typename T, int LPR, int NW, int NV, int TPB>
 static bool try_norm_bwd(const NormShape& s, const NormArgs& a, hipStream_t st) {
     if (s.lpr != LPR || s.nw != NW || s.nv != NV || s.tpb != TPB) return false;
-    norm_bwd_kernel<T, LPR, NW, NV, TPB><<<a.blocks, TPB, 0, st>>>(a);
+    // 32 values a lane do not fit its registers, least of all in float32, whose row on its way is as large as the one in work
+    // (1500 x 16384 f32: 126 us all in registers, 102 with the weights in LDS, 76 with dw too; 4000 x 12288 bf16: 79, 72, 72)
+    constexpr int KEEP = NV * Piece<T>::N < 32 ? 0 : Piece<T>::N == 4 ? 2 : 1;
+    norm_bwd_kernel<T, LPR, NW, NV, TPB, KEEP><<<a.blocks, TPB, 0, st>>>(a);
     return true;
 }
 

@@ -460,7 +460,16 @@ __device__ __forceinline__ void write_best(const ScoreArgs& a, int64_t r, const 
 // blocks of 256 threads that a unit holds at once
 constexpr int score_fwd_blocks(bool top) { return top ? 6 : 8; }
 
-// NW waves a slice of a row; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best keys.
+// One pass over a slice of a row: each thread keeps the largest score and the two sums of its pieces against it, a group's threads
+// meet at the end.  NW waves a slice; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best
+// keys.
+//
+// Bound by reading: 2048 x 131072 bf16 in 96 us, 5.6 TB/s (a large copy moves 5.2); 65536 x 1001 f32, a wave a row, in 54 us, 4.9
+// TB/s.  A score takes nine instructions (unpack, half a max3, subtract, multiply, exp2 as four, add; the entropy two more), which
+// is 60 % of the vector unit at that rate: the maximum is taken over two pieces at once so that moving the sums to it costs a
+// sixteenth, and nothing else is done per score.  Short of that: what a row costs beside its scores (8191 x 5382 f16 20 us, 4.4
+// TB/s) and, with 50 alternatives of 256 x 1e6 bf16, 114 us for 95: the slices' searches come at the same time, at their ends, their
+// second reads are a fifth of the first, and 9 of it are score_join_kernel.
 template <typename T, int NW, bool ENT, bool TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB, score_fwd_blocks(TOP)) score_fwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
@@ -536,7 +545,8 @@ __global__ void __launch_bounds__(SC_TPB, score_fwd_blocks(TOP)) score_fwd_kerne
     }
 }
 
-// a row's slices together: thread t holds slice t, its keys are in order
+// A row's slices together: thread t holds slice t, its keys are in order.  A chain of latencies: two loads, the cut, two more loads
+// and the ordering, 7 us for 244 slices with 20 keys each, 2.5 us without alternatives.
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
     __shared__ float scratch[3 * SC_NW];
@@ -625,7 +635,8 @@ __global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
 //
 // What a row costs beside reading it — maxima and sums across lanes, the ids, the writes — is the same instructions for one row or
 // for the 64 / LPR rows that a wave holds side by side.  A lane keeps P pieces; the piece that crosses the row's end is pulled
-// back into it, as in layer_norm.hip.
+// back into it, as in layer_norm.hip.  Bound by those instructions: 131072 x 64 f32 forward in 12 us (2.8 TB/s), backward in 23
+// (2.9 TB/s); 50000 x 10 f32 in 6 us each, which is little more than an empty launch.
 
 template <typename T, int LPR, int P>
 struct ShortRow {
@@ -1014,6 +1025,9 @@ static int launch_scores(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
 // slot of an id adds up all of them in order, so nothing depends on who comes first.  NW waves a slice; NW = 1: four rows a block.
 // List of a group in LDS: n16 ids (padded with -1 to whole sixteens), then n16 addends.  The first pieces and the list are on their
 // way at the same time.
+//
+// Bound by reading and writing: 2048 x 131072 bf16 in 193 us, 5.6 TB/s; 65536 x 1001 f32 with the entropy's part in 109 us, 4.8 TB/s.
+// A long list is compared with itself (4096 x 5382 bf16: 20 us with one id a row, 25 with 64, 34 with 100).
 template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_BWD_UNROLL;
