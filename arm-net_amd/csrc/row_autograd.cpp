@@ -3,8 +3,9 @@
 // The kernels and the C entries are layer_norm.hip's and score_rows.hip's; here is what a call on torch tensors does around them:
 // rows by strides, outputs, workspaces, the current stream, and the backward as a node of the graph.  It is C++ because of the
 // backward: that runs on the engine's own thread, and for a small batch a Python backward costs more there than both kernels (a
-// 64 x 5382 distillation step: 97 us with the nodes in Python).  The entries are bound by address from the library that the Python
-// package has loaded, so there is one copy of the kernels and one place that decides which library that is.
+// 64 x 5382 distillation step, whose kernels take 9 us: 97 us with the nodes in Python, 50 with these).  The entries are bound by
+// address from the library that the Python package has loaded, so there is one copy of the kernels and one place that decides
+// which library that is.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
