@@ -85,9 +85,10 @@ struct Columns {
             for (int e = 0; e < V; ++e) f[e] = e >= lo[i] ? f[e] : 0.f;
         }
     }
+    __device__ __forceinline__ bool whole(int i) const { return NT == 1 ? !tiny : lo[i] == 0; }
     __device__ __forceinline__ bool has(int i, int e) const { return NT == 1 ? !tiny || e < d : e >= lo[i]; }
     __device__ __forceinline__ void store(T* row, int i, const float (&f)[V]) const {
-        if (NT == 1 ? !tiny : lo[i] == 0) {
+        if (whole(i)) {
             Piece<T>::store(row + off[i], Piece<T>::pack(f));
         } else {
 #pragma unroll
@@ -224,9 +225,10 @@ struct LaneCells {
 };
 
 // dx of a row, and the block's share of dw and db: in registers over its rows, then over its groups through LDS.  x and dy are read
-// once for all three.  Bound by memory: with the sum over the blocks 65536 x 512 f32 in 82 us (4.9 TB/s), 16384 x 4096 bf16 in 80 (5.0);
-// of more than 8192 values less (1500 x 16384 f32 in 76, 3.9 TB/s): one row a CU is in work, one on its way.  A few hundred long rows
-// cost what the blocks' shares cost (1000 x 10000 bf16: 36 us, of which the rows 12).
+// once for all three.  Bound by memory: with the sum over the blocks 65536 x 512 f32 in 81 us (5.0 TB/s), 16384 x 4096 bf16 in 77 (5.2),
+// 8000 x 8192 bf16 in 79 (5.0); of more than 8192 values less (1500 x 16384 f32 in 70, 4.2 TB/s): one row a CU is in work, one on its
+// way.  A few hundred long rows cost what the blocks' shares cost (1000 x 10000 bf16: 26 us, of which the rows 12; 35 with the shares
+// stored value by value).
 // KEEP: what waits in LDS between the rows instead of in registers: 0 nothing, 1 the weights, 2 the sums for dw too.
 template <typename T, int LPR, int NW, int NV, int TPB, int KEEP>
 __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
@@ -360,19 +362,28 @@ __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
     }
     if (share == SHARES - 1) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float* part = a.partial + (int64_t)blockIdx.x * 2 * a.d + cols.off[i];
+            if (a.blocks > 1 && cols.whole(i)) {
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    Piece<float>::store(part + e, Piece<float>::pack(*(float(*)[4])(dw[i] + e)));
+                    Piece<float>::store(part + a.d + e, Piece<float>::pack(*(float(*)[4])(db[i] + e)));
+                }
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int col = cols.off[i] + e;
                 if (!cols.has(i, e)) continue;
                 if (a.blocks == 1) {
-                    if (a.dweight) store_param(a.dweight, a.w_type, col, dw[i][e]);
-                    if (a.dbias) store_param(a.dbias, a.w_type, col, db[i][e]);
+                    if (a.dweight) store_param(a.dweight, a.w_type, cols.off[i] + e, dw[i][e]);
+                    if (a.dbias) store_param(a.dbias, a.w_type, cols.off[i] + e, db[i][e]);
                 } else {
-                    a.partial[((int64_t)blockIdx.x * 2 + 0) * a.d + col] = dw[i][e];
-                    a.partial[((int64_t)blockIdx.x * 2 + 1) * a.d + col] = db[i][e];
+                    part[e] = dw[i][e];
+                    part[a.d + e] = db[i][e];
                 }
             }
+        }
     }
 }
 
@@ -632,7 +643,7 @@ template <typename T, int LPR, int NW, int NV, int TPB>
 static bool try_norm_bwd(const NormShape& s, const NormArgs& a, hipStream_t st) {
     if (s.lpr != LPR || s.nw != NW || s.nv != NV || s.tpb != TPB) return false;
     // 32 values a lane do not fit its registers, least of all in float32, whose row on its way is as large as the one in work
-    // (1500 x 16384 f32: 126 us all in registers, 102 with the weights in LDS, 76 with dw too; 4000 x 12288 bf16: 79, 72, 72)
+    // (1500 x 16384 f32: the weights in LDS take 24 us off, dw another 26; 4000 x 12288 bf16: 7 and 0)
     constexpr int KEEP = NV * Piece<T>::N < 32 ? 0 : Piece<T>::N == 4 ? 2 : 1;
     norm_bwd_kernel<T, LPR, NW, NV, TPB, KEEP><<<a.blocks, TPB, 0, st>>>(a);
     return true;
