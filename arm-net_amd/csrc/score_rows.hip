@@ -53,6 +53,7 @@ struct ScoreArgs {
     // a row in several slices
     int splits;
     int64_t per;               // scores of a slice
+    int slots;                 // of a long list's table
     float4* part;              // [rows, splits]: m, S, W
     uint64_t* keys;            // [rows, splits, top], best first; 0: none
 };
@@ -1021,21 +1022,65 @@ static int launch_scores(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_t s
     return a.top ? launch_score_fwd<T, false, true, false>(a, ws, ws_bytes, st) : launch_score_fwd<T, false, false, false>(a, ws, ws_bytes, st);
 }
 
-// The gradient of a slice of a row: p's part of it everywhere, then the listed ids' values again with what they add.  The first
-// slot of an id adds up all of them in order, so nothing depends on who comes first.  NW waves a slice; NW = 1: four rows a block.
-// List of a group in LDS: n16 ids (padded with -1 to whole sixteens), then n16 addends.  The first pieces and the list are on their
-// way at the same time.
+// A long list, each of its ids once: add(id, sum of its addends), from one lane of the group.  The slots' numbers go into an open
+// table by their ids (a power of two, a fifth larger than the list at least, -1 where empty); the slot that is there keeps the id and
+// is marked if another one comes.  Which one that is may differ from run to run; the sum does not: a wave adds up a marked id's
+// addends from the whole list, in an order that their places fix.
+constexpr int32_t MORE = 1 << 30;
+
+template <int NW, typename F>
+__device__ __forceinline__ void add_listed(const int32_t* s_id, const float* s_g, int n, int32_t* table, int slots, int tid, F add) {
+    constexpr int NT = NW * WAVE;
+    const int lane = tid & (WAVE - 1);
+    for (int k = tid; k < n; k += NT) {
+        const int32_t id = s_id[k];
+        if (id < 0) continue;
+        uint32_t h = (uint32_t)id * 2654435769u >> 16;            // Knuth's multiplicative hash
+        for (;;) {                                                // ends: the table has empty places
+            h &= (uint32_t)slots - 1;
+            const int32_t there = atomicCAS(table + h, -1, k);
+            if (there == -1) break;
+            if (s_id[there & ~MORE] == id) {
+                atomicOr(table + h, MORE);
+                break;
+            }
+            ++h;
+        }
+    }
+    group_sync<NW>();
+    for (int h = tid; h < slots; h += NT) {                       // whole waves
+        const int32_t k = table[h];
+        const int32_t id = k == -1 ? -1 : s_id[k & ~MORE];
+        float g = k == -1 ? 0.f : s_g[k & ~MORE];
+        for (uint64_t more = __ballot(k != -1 && (k & MORE)); more; more &= more - 1) {
+            const int l = __builtin_ctzll(more);
+            const int32_t its = __builtin_amdgcn_readlane(id, l);
+            float part = 0.f;
+            for (int i = lane; i < n; i += WAVE) part += s_id[i] == its ? s_g[i] : 0.f;
+            part = wave_sum(part);
+            if (lane == l) g = part;
+        }
+        if (id >= 0) add(id, g);
+    }
+}
+
+// The gradient of a slice of a row: p's part of it everywhere, then the listed ids' values again with what they add.  Of a
+// list of up to 64 every slot looks at all others, and the first one of an id adds them up in order; a longer one has a table.  NW
+// waves a slice; NW = 1: four rows a block.  List of a group in LDS: n16 ids (padded with -1 to whole sixteens), n16 addends, the
+// table.  The first pieces and the list are on their way at the same time.
 //
 // Bound by reading and writing: 2048 x 131072 bf16 in 193 us, 5.6 TB/s; 65536 x 1001 f32 with the entropy's part in 109 us, 4.8 TB/s.
-// A long list is compared with itself (4096 x 5382 bf16: 20 us with one id a row, 25 with 64, 34 with 100).
+// 4096 x 5382 bf16 in 20 us with one id a row, 25 with 64, 27 with 100, 48 with 200, 167 with 1024 (compared with each other
+// 34, 67 and 979): what is left is the ids that come twice.
 template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_BWD_UNROLL;
     extern __shared__ int4 lists[];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x & (NT - 1), lane = tid & (WAVE - 1);
     const int n16 = (a.n_ids + 15) & ~15;
-    int32_t* s_id = (int32_t*)lists + group * 2 * n16;
+    int32_t* s_id = (int32_t*)lists + group * (2 * n16 + a.slots);
     float* s_g = (float*)(s_id + n16);
+    int32_t* table = s_id + 2 * n16;                    // [slots], none for a short list
     const int64_t units = a.rows * a.splits;
     for (int64_t unit = (int64_t)blockIdx.x * GROUPS + group; unit < units; unit += (int64_t)gridDim.x * GROUPS) {
         const int64_t back = units - 1 - unit;          // the forward's last rows first: some are still in the last-level cache
@@ -1062,6 +1107,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         bool used = false;
         int32_t first = -1;                             // this thread's slot of the list (k = tid), its addend and the row's score
         float first_g = 0.f, first_x = 0.f;
+        for (int h = tid; h < a.slots; h += NT) table[h] = -1;
         for (int k0 = 0; k0 < n16; k0 += WAVE) {        // every wave adds up the whole list, each keeps its share of it
             const int k = k0 + lane;
             int32_t at = -1;
@@ -1131,16 +1177,14 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
         // the list is complete, and the stores above come before the ones below
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         group_sync<NW>();
-        for (int k = tid; k < a.n_ids; k += NT) {
-            if (k != tid) {
-                first = s_id[k];
-                if (first >= 0) {
-                    first_g = s_g[k];
-                    first_x = to_f32(x[first]);
-                }
-            }
+        if (a.slots) {
+            add_listed<NW>(s_id, s_g, n16, table, a.slots, tid, [&](int32_t id, float g) {
+                dx[id] = from_f32<T>(fmaf(g, u, base(to_f32(x[id]))));
+            });
+            continue;
+        }
+        if (tid < a.n_ids && first >= 0) {
             const int32_t id = first;
-            if (id < 0) continue;
             float g = first_g;
             int same = 0;
             for (int i = 0; i < n16; i += 16)
@@ -1150,7 +1194,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
                     same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
                 }
             if (same > 1) {                             // the first of them adds them all up, in order
-                int lead = k;
+                int lead = tid;
                 g = 0.f;
                 for (int i = 0; i < n16; i += 16)
 #pragma unroll
@@ -1159,7 +1203,7 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
                         lead = is && i + q < lead ? i + q : lead;
                         g += is ? s_g[i + q] : 0.f;
                     }
-                if (lead != k) continue;
+                if (lead != tid) continue;
             }
             dx[id] = from_f32<T>(fmaf(g, u, base(first_x)));
         }
@@ -1185,7 +1229,11 @@ static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
     if (narrow) splits = 1;
     a.per = splits == 1 ? a.c : ((a.c + splits - 1) / splits + 63) / 64 * 64;
     a.splits = (int)((a.c + a.per - 1) / a.per);
-    const size_t list = (size_t)((a.n_ids + 15) & ~15) * 8;
+    const int n16 = (a.n_ids + 15) & ~15;
+    a.slots = 0;
+    if (a.n_ids > WAVE)
+        for (a.slots = 128; a.slots < n16 + n16 / 5;) a.slots *= 2;
+    const size_t list = (size_t)(2 * n16 + a.slots) * 4;          // four of them: at most 64 KiB
     if (narrow)
         score_bwd_kernel<T, 1, ENT, DISTILL><<<row_grid((a.rows + 3) / 4), SC_TPB, 4 * list, st>>>(a);
     else

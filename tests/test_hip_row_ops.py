@@ -349,6 +349,31 @@ def test_long_lists_of_ids(n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,c", [(5, 1500), (9000, 600), (7, 6001), (3, 50001)])
+@pytest.mark.parametrize("n", [63, 65, 129, 1000, 1024])
+def test_long_lists_of_ids_on_longer_rows(n, rows, c, dtype):
+    """ids that are alone, several times, everywhere or nowhere in the list; the same bits again"""
+    rows = rows if n < 1000 else min(rows, 40)
+    x = rnd(rows, c).to(dtype)
+    ids = torch.randint(-1, c, (rows, n), generator=gen(1))
+    ids[1, ::2] = c - 1
+    ids[2] = 7
+    ids[-1, :n // 2] = torch.arange(n // 2) * 5 % c              # neighbours in the list are neighbours in the row
+    if rows > 3:
+        ids[3] = -1
+        ids[4] = torch.randint(0, 9, (n,), generator=gen(4))
+    g = rnd(rows, n, seed=2)
+    xd = x.to(DEV).requires_grad_(True)
+    logp = score_logprobs(xd, ids.to(DEV), check_ids=False).logp
+    got, = torch.autograd.grad(logp, xd, g.to(DEV), retain_graph=True)
+    dx, size = scores_grad_ref(x, ids, 1.0, g, None)
+    close(got, dx, half_step(dtype, dx) + (n + 2 * chain(c) + 4 * z_size(x, 1.0)) * U * size)
+    for _ in range(3):
+        again, = torch.autograd.grad(logp, xd, g.to(DEV), retain_graph=True)
+        assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_scores_take_rows_where_they_are(dtype):
     base = (rnd(4, 5, 301) * 2).to(dtype).to(DEV)
     for v in (base[..., 1:], base[:, 1:, :-1], base[:, :-1], base.transpose(0, 1)[..., 3:], base[1, 2, 1:], base[0, :1, 1:].expand(3, 300),
