@@ -865,11 +865,11 @@ __global__ void __launch_bounds__(SC_TPB) score_short_bwd_kernel(ScoreArgs a) {
             float g = 0.f;
             if (k0 + tid < a.n_ids) {
                 const int64_t k = r * a.n_ids + k0 + tid, id = load_id(a.ids, a.id_type, k);
+                const float given = DISTILL ? load_any(a.teacher, a.t_type, k) : a.g_logp ? a.g_logp[k] : 0.f;     // beside the id
                 if (id >= 0 && id < a.c && !none) {
                     at = (int)id;
                     used = 1.f;
-                    if (DISTILL) g = exp2_raw((load_any(a.teacher, a.t_type, k) - mt) * a.c2 - lt);
-                    else if (a.g_logp) g = a.g_logp[k];
+                    g = DISTILL ? exp2_raw((given - mt) * a.c2 - lt) : given;
                     sum += g;
                 }
             }
@@ -1069,8 +1069,9 @@ __device__ __forceinline__ void add_listed(const int32_t* s_id, const float* s_g
 // waves a slice; NW = 1: four rows a block.  List of a group in LDS: n16 ids (padded with -1 to whole sixteens), n16 addends, the
 // table.  The first pieces and the list are on their way at the same time.
 //
-// Bound by reading and writing: 2048 x 131072 bf16 in 193 us, 5.6 TB/s; 65536 x 1001 f32 with the entropy's part in 109 us, 4.8 TB/s.
-// 4096 x 5382 bf16 in 20 us with one id a row, 25 with 64, 27 with 100, 48 with 200, 167 with 1024 (compared with each other
+// Bound by reading and writing: 2048 x 131072 bf16 in 193 us, 5.6 TB/s; 65536 x 1001 f32 with the entropy's part in 108 us, 4.9 TB/s
+// (112 with an addend's load behind its id's).
+// 4096 x 5382 bf16 in 19 us with one id a row, 25 with 64, 26 with 100, 48 with 200, 167 with 1024 (compared with each other
 // 34, 67 and 979): what is left is the ids that come twice.
 template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
@@ -1114,14 +1115,13 @@ __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
             float g = 0.f;
             if (k < a.n_ids) {
                 const int64_t id = load_id(a.ids, a.id_type, r * a.n_ids + k);
+                if (DISTILL) g = load_any(a.teacher, a.t_type, r * a.n_ids + k);          // beside the id
+                else if (a.g_logp) g = a.g_logp[r * a.n_ids + k];
                 const bool in = id >= 0 && id < a.c && !none;
                 used = used || in;
-                if (DISTILL) {
-                    if (in) g = exp2_raw((load_any(a.teacher, a.t_type, r * a.n_ids + k) - mt) * a.c2 - lt);
-                } else if (in && a.g_logp) {
-                    g = a.g_logp[r * a.n_ids + k];
-                    sum += g;
-                }
+                if (DISTILL) g = exp2_raw((g - mt) * a.c2 - lt);
+                g = in ? g : 0.f;
+                sum += g;
                 if (in && id >= from && id < from + n) at = (int32_t)id - from;
             }
             if (k < n16 && (k0 / WAVE) % NW == tid / WAVE) {
