@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
             for (int e = 0; e < V; ++e) s += f[i][e];
         }
         if (k + 1 < rounds) cols.load(row_ptr<T>(a.x, r + step < a.rows ? r + step : a.rows - 1), raw);
-        const float mean = row_sum<LPR, NW>(s, scratch[0]) / (float)a.d;     // a constant row is its own mean
+        const float mean = row_sum<LPR, NW>(s, scratch[0]) / (float)a.d;     // a division: one rounding less
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
