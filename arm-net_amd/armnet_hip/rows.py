@@ -4,7 +4,8 @@ A row is the last dimension of a tensor: a sample's features in front of a proje
 behind one.  `layer_norm` stands beside the training BatchNorm (it needs no batch statistics: a batch of one, a sharded
 server), `score_logprobs` and `distill_loss` beside the sparse map over a row of scores: what a row answers, and what a
 student learns from a teacher's answer.  Device tensors run the HIP kernels (float32, bfloat16, float16; fp32 arithmetic),
-host tensors the same formulas on ATen ops.  All three are differentiable once.
+host tensors the same formulas on ATen ops.  All three are differentiable once, by a backward pass; an input with a
+forward-mode tangent is refused.
 """
 from typing import NamedTuple, Optional
 

@@ -151,6 +151,13 @@ variable_list once(variable_list grads, const char* name) {
     return grads;
 }
 
+// A tangent (forward-mode derivative) cannot pass the kernels; a result without one would be taken for a constant.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->_fw_grad(0).defined())
+            throw ArmnetError(std::string(name) + ": forward-mode derivatives are not supported (use the backward pass)");
+}
+
 bool wants_graph(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------------
@@ -186,6 +193,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Tensor &x_ = saved[0], &weight = saved[1], &st = saved[2];
         const int64_t need = ctx->saved_data["need"].toInt();
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        refuse_tangents("layer_norm's backward", {&grads[0]});
         OnDevice on(x_);
         const Rows x = rows_of(x_);
         const Tensor dy = grads[0].contiguous();
@@ -204,8 +212,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
-    if (wants_graph(x) || wants_graph(or_none(weight)) || wants_graph(or_none(bias))) return LayerNorm::apply(x, weight, bias, eps);
-    return norm_forward(x, or_none(weight), or_none(bias), eps, false).first;
+    const Tensor w = or_none(weight), b = or_none(bias);
+    refuse_tangents("layer_norm", {&x, &w, &b});
+    if (wants_graph(x) || wants_graph(w) || wants_graph(b)) return LayerNorm::apply(x, weight, bias, eps);
+    return norm_forward(x, w, b, eps, false).first;
 }
 
 // ---- log probabilities ---------------------------------------------------------------------------------------------------
@@ -267,6 +277,7 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
         Tensor g_logp, g_entropy, dx;
         if (has & 1) g_logp = grads[0];
         if (has & 2) g_entropy = grads[has & 1];
+        refuse_tangents("score_logprobs' backward", {&g_logp, &g_entropy});
         if (g_logp.defined()) g_logp = g_logp.contiguous();
         if (g_entropy.defined()) g_entropy = g_entropy.contiguous();
         if (g_logp.defined() || g_entropy.defined()) {
@@ -286,6 +297,7 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
 
 std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(const Tensor& X, const MaybeTensor& ids, double temperature,
                                                                               int64_t top, bool entropy, const MaybeTensor& word) {
+    refuse_tangents("score_logprobs", {&X});
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     if (wants_graph(X) && (ids.has_value() || entropy || top)) {
         const variable_list out = ScoreLogprobs::apply(X, ids, temperature, top, entropy, word);
@@ -332,6 +344,7 @@ struct Distill : torch::autograd::Function<Distill> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &X_ = saved[0], &ids = saved[1], &teacher = saved[2], &st = saved[3];
+        refuse_tangents("distill_loss' backward", {&grads[0]});
         OnDevice on(X_);
         const Rows X = rows_of(X_);
         const Tensor g = grads[0].contiguous();
@@ -346,6 +359,7 @@ struct Distill : torch::autograd::Function<Distill> {
 };
 
 Tensor distill_loss(const Tensor& X, const Tensor& ids, const Tensor& teacher, double temperature, const MaybeTensor& word) {
+    refuse_tangents("distill_loss", {&X, &teacher});
     if (wants_graph(X)) return Distill::apply(X, ids, teacher, temperature, word);
     return distill_forward(X, ids, teacher, temperature, false, or_none(word)).first;
 }

@@ -1,0 +1,49 @@
+"""What the row operators refuse on the device through their public entries, and that nothing else changes by it."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd_ad
+
+from armnet_hip import HipDistillLoss, HipLayerNorm, HipScoreLogprobs, distill_loss, layer_norm, native, score_logprobs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+Error = native.ArmnetNativeError
+
+
+def inputs(n=5, c=40, k=3):
+    g = torch.Generator().manual_seed(0)
+    return (torch.randn(n, c, generator=g).to(DEV), torch.randn(c, generator=g).to(DEV),
+            torch.randint(0, c, (n, k), generator=g).to(DEV), torch.randn(n, k, generator=g).to(DEV))
+
+
+@pytest.mark.parametrize("c", [40, 20001])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_forward_mode_is_refused(c, reverse):
+    x, w, ids, ts = inputs(c=c)
+    norm = HipLayerNorm(c).to(DEV)
+    with fwd_ad.dual_level():
+        dual = lambda t: fwd_ad.make_dual(t.clone().requires_grad_(reverse), torch.ones_like(t))      # noqa: E731
+        for call in (lambda: layer_norm(dual(x)), lambda: layer_norm(x, dual(w)), lambda: layer_norm(x, None, dual(w)),
+                     lambda: norm(dual(x)), lambda: score_logprobs(dual(x), ids), lambda: score_logprobs(dual(x), entropy=True),
+                     lambda: score_logprobs(dual(x), top_k=2), lambda: HipScoreLogprobs(entropy=True)(dual(x)),
+                     lambda: distill_loss(dual(x), ids, ts), lambda: HipDistillLoss()(dual(x), ids, ts)):
+            with pytest.raises(Error, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode|constant"):
+            distill_loss(x, ids, fwd_ad.make_dual(ts, torch.ones_like(ts)))
+        assert layer_norm(x, w).isfinite().all()                 # the level alone is no reason
+
+
+@pytest.mark.parametrize("c", [40, 20001])
+def test_a_tangent_of_the_upstream_gradient_is_refused(c):
+    x, w, ids, ts = inputs(c=c)
+    x.requires_grad_(True)
+    calls = (lambda: layer_norm(x, w), lambda: score_logprobs(x, ids).logp, lambda: score_logprobs(x, ids, entropy=True).entropy,
+             lambda: distill_loss(x, ids, ts))
+    for call in calls:
+        out = call()
+        want, = torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+        with fwd_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, fwd_ad.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
+        assert torch.equal(torch.autograd.grad(out, x, torch.ones_like(out))[0], want)

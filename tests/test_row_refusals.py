@@ -1,0 +1,52 @@
+"""What the row operators' C++ calls refuse before anything else, so that it shows without a GPU: on a host tensor a call that is not
+refused for its reason ends at `expected a tensor on the HIP device`."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd_ad
+
+from armnet_hip import distill_loss, layer_norm, native, score_logprobs
+
+Error = native.ArmnetNativeError
+
+
+def calls(tensor):
+    """every call, with each of its float inputs in turn made by `tensor(shape)`"""
+    rows = native.rows()
+    x, w, ids, ts = torch.randn(3, 8), torch.randn(8), torch.zeros(3, 2, dtype=torch.int64), torch.randn(3, 2)
+    return {
+        "layer_norm(x)": lambda: rows.layer_norm(tensor(3, 8), w, w, 1e-5),
+        "layer_norm(weight)": lambda: rows.layer_norm(x, tensor(8), None, 1e-5),
+        "layer_norm(bias)": lambda: rows.layer_norm(x, None, tensor(8), 1e-5),
+        "score_logprobs(X)": lambda: rows.score_logprobs(tensor(3, 8), ids, 1.0, 2, True, None),
+        "score_logprobs(X) without ids": lambda: rows.score_logprobs(tensor(3, 8), None, 1.0, 0, True, None),
+        "distill_loss(X)": lambda: rows.distill_loss(tensor(3, 8), ids, ts, 1.0, None),
+        "distill_loss(top_scores)": lambda: rows.distill_loss(x, ids, tensor(3, 2), 1.0, None),
+    }
+
+
+NAMES = list(calls(torch.randn))
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_forward_mode_is_refused(name, reverse):
+    """a tangent that the kernels cannot carry is no result without one"""
+    with fwd_ad.dual_level():
+        with pytest.raises(Error, match="forward-mode"):
+            calls(lambda *s: fwd_ad.make_dual(torch.randn(s).requires_grad_(reverse), torch.ones(s)))[name]()
+        with torch.no_grad(), pytest.raises(Error, match="forward-mode"):          # no_grad is about the other mode
+            calls(lambda *s: fwd_ad.make_dual(torch.randn(s), torch.ones(s)))[name]()
+        with pytest.raises(Error, match="HIP device"):                             # the level alone is no reason
+            calls(torch.randn)[name]()
+
+
+def test_forward_mode_is_refused_on_host():
+    ids, ts = torch.zeros(3, 2, dtype=torch.int64), torch.randn(3, 2)
+    with fwd_ad.dual_level():
+        x, w = fwd_ad.make_dual(torch.randn(3, 8), torch.ones(3, 8)), fwd_ad.make_dual(torch.randn(8), torch.ones(8))
+        t = fwd_ad.make_dual(ts, torch.ones(3, 2))
+        for call in (lambda: layer_norm(x), lambda: layer_norm(torch.randn(3, 8), w), lambda: score_logprobs(x, ids),
+                     lambda: score_logprobs(x, entropy=True), lambda: distill_loss(x, ids, ts),
+                     lambda: distill_loss(torch.randn(3, 8), ids, t)):
+            with pytest.raises(RuntimeError):
+                call()
