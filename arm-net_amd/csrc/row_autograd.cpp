@@ -8,9 +8,11 @@
 // which library that is.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "../../include/armnet_hip.h"
 
@@ -151,8 +153,12 @@ variable_list once(variable_list grads, const char* name) {
     return grads;
 }
 
-// A tangent (forward-mode derivative) cannot pass the kernels; a result without one would be taken for a constant.
-void refuse_tangents(const char* name, std::initializer_list<const Tensor*> inputs) {
+// What a call cannot do.  A tangent (forward-mode derivative) cannot pass the kernels; a result without one would be taken for a
+// constant.  A trace records the outputs' allocation and not the kernels; what it replays would be memory that nothing wrote.
+void refuse(const char* name, std::initializer_list<const Tensor*> inputs) {
+    using c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
+        throw ArmnetError(std::string(name) + ": a trace cannot record the kernels (call it outside of the traced part)");
     for (const Tensor* t : inputs)
         if (t->defined() && t->_fw_grad(0).defined())
             throw ArmnetError(std::string(name) + ": forward-mode derivatives are not supported (use the backward pass)");
@@ -193,7 +199,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Tensor &x_ = saved[0], &weight = saved[1], &st = saved[2];
         const int64_t need = ctx->saved_data["need"].toInt();
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
-        refuse_tangents("layer_norm's backward", {&grads[0]});
+        refuse("layer_norm's backward", {&grads[0]});
         OnDevice on(x_);
         const Rows x = rows_of(x_);
         const Tensor dy = grads[0].contiguous();
@@ -213,7 +219,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
     const Tensor w = or_none(weight), b = or_none(bias);
-    refuse_tangents("layer_norm", {&x, &w, &b});
+    refuse("layer_norm", {&x, &w, &b});
     if (wants_graph(x) || wants_graph(w) || wants_graph(b)) return LayerNorm::apply(x, weight, bias, eps);
     return norm_forward(x, w, b, eps, false).first;
 }
@@ -277,7 +283,7 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
         Tensor g_logp, g_entropy, dx;
         if (has & 1) g_logp = grads[0];
         if (has & 2) g_entropy = grads[has & 1];
-        refuse_tangents("score_logprobs' backward", {&g_logp, &g_entropy});
+        refuse("score_logprobs' backward", {&g_logp, &g_entropy});
         if (g_logp.defined()) g_logp = g_logp.contiguous();
         if (g_entropy.defined()) g_entropy = g_entropy.contiguous();
         if (g_logp.defined() || g_entropy.defined()) {
@@ -297,7 +303,7 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
 
 std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(const Tensor& X, const MaybeTensor& ids, double temperature,
                                                                               int64_t top, bool entropy, const MaybeTensor& word) {
-    refuse_tangents("score_logprobs", {&X});
+    refuse("score_logprobs", {&X});
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     if (wants_graph(X) && (ids.has_value() || entropy || top)) {
         const variable_list out = ScoreLogprobs::apply(X, ids, temperature, top, entropy, word);
@@ -344,7 +350,7 @@ struct Distill : torch::autograd::Function<Distill> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &X_ = saved[0], &ids = saved[1], &teacher = saved[2], &st = saved[3];
-        refuse_tangents("distill_loss' backward", {&grads[0]});
+        refuse("distill_loss' backward", {&grads[0]});
         OnDevice on(X_);
         const Rows X = rows_of(X_);
         const Tensor g = grads[0].contiguous();
@@ -359,7 +365,7 @@ struct Distill : torch::autograd::Function<Distill> {
 };
 
 Tensor distill_loss(const Tensor& X, const Tensor& ids, const Tensor& teacher, double temperature, const MaybeTensor& word) {
-    refuse_tangents("distill_loss", {&X, &teacher});
+    refuse("distill_loss", {&X, &teacher});
     if (wants_graph(X)) return Distill::apply(X, ids, teacher, temperature, word);
     return distill_forward(X, ids, teacher, temperature, false, or_none(word)).first;
 }

@@ -47,3 +47,24 @@ def test_a_tangent_of_the_upstream_gradient_is_refused(c):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, x, fwd_ad.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
         assert torch.equal(torch.autograd.grad(out, x, torch.ones_like(out))[0], want)
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tracing_is_refused(requires_grad):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, ids, ts = inputs()
+    norm, scores, loss = HipLayerNorm(40).to(DEV), HipScoreLogprobs(top_k=2, entropy=True), HipDistillLoss()
+    a = x.clone().requires_grad_(requires_grad)
+    for f in (lambda a: layer_norm(a, w), norm, lambda a: score_logprobs(a, ids, check_ids=False).logp, lambda a: scores(a, ids).top_logp,
+              lambda a: distill_loss(a, ids, ts, check_ids=False), lambda a: loss(a, ids, ts)):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, a, check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(f)(x)
+        f(x)                                                     # not recorded: as ever
+
+
+def test_a_compiled_program_runs_around_the_kernels():
+    x, w, ids, ts = inputs()
+    f = lambda a: layer_norm(a * 2, w) + score_logprobs(a, ids, check_ids=False).logp.sum()      # noqa: E731
+    assert torch.equal(torch.compile(f, backend="eager")(x), f(x))

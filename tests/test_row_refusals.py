@@ -50,3 +50,29 @@ def test_forward_mode_is_refused_on_host():
                      lambda: distill_loss(torch.randn(3, 8), ids, t)):
             with pytest.raises(RuntimeError):
                 call()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(name):
+    """a recorder sees the outputs' allocation and not the kernels: what it replays is memory that nothing wrote"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def run(a):
+        return calls(lambda *s: a[0] if len(s) == 1 else a[:s[0], :s[1]])[name]()
+
+    a = torch.randn(3, 8)
+    for requires_grad in (False, True):
+        with pytest.raises(Error, match="trace"):
+            torch.jit.trace(run, a.requires_grad_(requires_grad), check_trace=False)
+    with pytest.raises(Error, match="trace"):
+        make_fx(run)(a.detach())
+    with pytest.raises(Error, match="HIP device"):
+        run(a)
+
+
+def test_host_tensors_can_be_traced():
+    x, ids = torch.randn(3, 8), torch.zeros(3, 2, dtype=torch.int64)
+    f = torch.jit.trace(lambda a: layer_norm(a) * 2, torch.randn(3, 8))
+    assert torch.equal(f(x), layer_norm(x) * 2)
+    f = torch.jit.trace(lambda a: score_logprobs(a, ids, check_ids=False).logp, torch.randn(3, 8))
+    assert torch.equal(f(x), score_logprobs(x, ids).logp)
