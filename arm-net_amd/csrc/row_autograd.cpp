@@ -155,13 +155,17 @@ variable_list once(variable_list grads, const char* name) {
 
 // What a call cannot do.  A tangent (forward-mode derivative) cannot pass the kernels; a result without one would be taken for a
 // constant.  A trace records the outputs' allocation and not the kernels; what it replays would be memory that nothing wrote.
+// A tensor without memory (a fake one, or one whose storage was freed) has its offset for an address.
 void refuse(const char* name, std::initializer_list<const Tensor*> inputs) {
     using c10::impl::TorchDispatchModeTLS;
     if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value())
         throw ArmnetError(std::string(name) + ": a trace cannot record the kernels (call it outside of the traced part)");
-    for (const Tensor* t : inputs)
-        if (t->defined() && t->_fw_grad(0).defined())
+    for (const Tensor* t : inputs) {
+        if (!t->defined()) continue;
+        if (t->_fw_grad(0).defined())
             throw ArmnetError(std::string(name) + ": forward-mode derivatives are not supported (use the backward pass)");
+        if (t->numel() && !t->storage().data()) throw ArmnetError(std::string(name) + ": a tensor without memory (fake, or its storage was freed)");
+    }
 }
 
 bool wants_graph(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
@@ -199,7 +203,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Tensor &x_ = saved[0], &weight = saved[1], &st = saved[2];
         const int64_t need = ctx->saved_data["need"].toInt();
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
-        refuse("layer_norm's backward", {&grads[0]});
+        refuse("layer_norm's backward", {&x_, &weight, &st, &grads[0]});
         OnDevice on(x_);
         const Rows x = rows_of(x_);
         const Tensor dy = grads[0].contiguous();
@@ -283,7 +287,7 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
         Tensor g_logp, g_entropy, dx;
         if (has & 1) g_logp = grads[0];
         if (has & 2) g_entropy = grads[has & 1];
-        refuse("score_logprobs' backward", {&g_logp, &g_entropy});
+        refuse("score_logprobs' backward", {&X_, &ids, &stats, &entropy, &g_logp, &g_entropy});
         if (g_logp.defined()) g_logp = g_logp.contiguous();
         if (g_entropy.defined()) g_entropy = g_entropy.contiguous();
         if (g_logp.defined() || g_entropy.defined()) {
@@ -303,7 +307,8 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
 
 std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(const Tensor& X, const MaybeTensor& ids, double temperature,
                                                                               int64_t top, bool entropy, const MaybeTensor& word) {
-    refuse("score_logprobs", {&X});
+    const Tensor list = or_none(ids);
+    refuse("score_logprobs", {&X, &list});
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     if (wants_graph(X) && (ids.has_value() || entropy || top)) {
         const variable_list out = ScoreLogprobs::apply(X, ids, temperature, top, entropy, word);
@@ -312,7 +317,7 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(co
         MaybeTensor logp = next(ids.has_value()), ent = next(entropy), tl = next(top), ti = next(top);
         return {logp, ent, tl, ti};
     }
-    const Answer o = scores_forward(X, or_none(ids), temperature, top, entropy, false, or_none(word));
+    const Answer o = scores_forward(X, list, temperature, top, entropy, false, or_none(word));
     return {some(o.logp), some(o.entropy), some(o.top_logp), some(o.top_ids)};
 }
 
@@ -350,7 +355,7 @@ struct Distill : torch::autograd::Function<Distill> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &X_ = saved[0], &ids = saved[1], &teacher = saved[2], &st = saved[3];
-        refuse("distill_loss' backward", {&grads[0]});
+        refuse("distill_loss' backward", {&X_, &ids, &teacher, &st, &grads[0]});
         OnDevice on(X_);
         const Rows X = rows_of(X_);
         const Tensor g = grads[0].contiguous();
@@ -365,7 +370,7 @@ struct Distill : torch::autograd::Function<Distill> {
 };
 
 Tensor distill_loss(const Tensor& X, const Tensor& ids, const Tensor& teacher, double temperature, const MaybeTensor& word) {
-    refuse("distill_loss", {&X, &teacher});
+    refuse("distill_loss", {&X, &ids, &teacher});
     if (wants_graph(X)) return Distill::apply(X, ids, teacher, temperature, word);
     return distill_forward(X, ids, teacher, temperature, false, or_none(word)).first;
 }

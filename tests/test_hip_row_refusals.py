@@ -68,3 +68,26 @@ def test_a_compiled_program_runs_around_the_kernels():
     x, w, ids, ts = inputs()
     f = lambda a: layer_norm(a * 2, w) + score_logprobs(a, ids, check_ids=False).logp.sum()      # noqa: E731
     assert torch.equal(torch.compile(f, backend="eager")(x), f(x))
+
+
+def test_a_storage_that_was_freed_is_refused():
+    """forward, and backward of what was saved; taken back, the same call runs"""
+    base, w, ids, ts = inputs(c=44)
+    x, w = base[:, 4:].detach().requires_grad_(True), w[4:].detach().requires_grad_(True)      # an offset of its own
+    ids = ids % 40
+    calls = (lambda a: layer_norm(a, w), lambda a: score_logprobs(a, ids, entropy=True).entropy, lambda a: distill_loss(a, ids, ts))
+    for call in calls:
+        want = call(x)
+        up = torch.ones_like(want)
+        grad, = torch.autograd.grad(want, x, up, retain_graph=True)
+        keep, storage = x.detach().clone(), x.untyped_storage()
+        size = storage.size()
+        storage.resize_(0)
+        for again in (lambda: call(x), lambda: call(x.detach()), lambda: torch.autograd.grad(want, x, up, retain_graph=True)):
+            with pytest.raises(RuntimeError, match="memory"):
+                again()
+        storage.resize_(size)
+        with torch.no_grad():
+            x.copy_(keep)
+        out = call(x)
+        assert torch.equal(out, want) and torch.equal(torch.autograd.grad(out, x, up)[0], grad)

@@ -76,3 +76,25 @@ def test_host_tensors_can_be_traced():
     assert torch.equal(f(x), layer_norm(x) * 2)
     f = torch.jit.trace(lambda a: score_logprobs(a, ids, check_ids=False).logp, torch.randn(3, 8))
     assert torch.equal(f(x), score_logprobs(x, ids).logp)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tensors_without_memory_are_refused(name):
+    """a fake view's address is an offset from nowhere"""
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode() as mode:
+        def fake(*s):
+            t = mode.from_tensor(torch.zeros(s[:-1] + (s[-1] + 4,)))[..., 4:]
+            assert t.storage_offset() == 4
+            return t
+        with pytest.raises(Error, match="memory"):
+            calls(fake)[name]()
+
+    def freed(*s):                                               # behind its tensors, as sharded parameters are
+        t = torch.zeros(s[:-1] + (s[-1] + 4,))[..., 4:]
+        t.untyped_storage().resize_(0)
+        return t
+    with pytest.raises(Error, match="memory"):
+        calls(freed)[name]()
+    with pytest.raises(Error, match="HIP device"):
+        calls(torch.randn)[name]()
