@@ -66,6 +66,10 @@ int id_type(const Tensor& t) {
 
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor or_none(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+// what memory holds is what the tensor says (a view that is negated on reading is copied)
+Tensor as_stored(const Tensor& t) { return t.defined() ? t.resolve_neg() : t; }
+MaybeTensor as_stored(const MaybeTensor& t) { return t.has_value() ? MaybeTensor(as_stored(*t)) : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? as_stored(t).contiguous() : t; }
 
 // The rows of a tensor as the C entries take them: row r begins (r / inner) * outer + (r % inner) * stride elements behind x
 // (inner = 0: r * stride).  Leading dimensions that two strides describe need no copy: slices, transposed batches, expanded rows.
@@ -74,9 +78,9 @@ struct Rows {
     int64_t n, inner = 0, outer = 0, stride, d;
 };
 
-Rows rows_of(const Tensor& t) {
+Rows rows_of(const Tensor& x) {
     Rows o;
-    o.x = t;
+    const Tensor t = o.x = as_stored(x);
     o.d = t.size(-1);
     o.n = t.numel() / o.d;
     o.stride = o.d;
@@ -206,7 +210,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         refuse("layer_norm's backward", {&x_, &weight, &st, &grads[0]});
         OnDevice on(x_);
         const Rows x = rows_of(x_);
-        const Tensor dy = grads[0].contiguous();
+        const Tensor dy = dense(grads[0]);
         Tensor dx, dw, db, ws;
         if (need & 1) dx = fresh(x.x, x.x.sizes(), x.x.scalar_type());
         if (need & 2) dw = fresh(x.x, {x.d}, type);
@@ -221,7 +225,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 };
 
-Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+Tensor layer_norm(const Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, double eps) {
+    const MaybeTensor weight = as_stored(weight_), bias = as_stored(bias_);
     const Tensor w = or_none(weight), b = or_none(bias);
     refuse("layer_norm", {&x, &w, &b});
     if (wants_graph(x) || wants_graph(w) || wants_graph(b)) return LayerNorm::apply(x, weight, bias, eps);
@@ -288,8 +293,8 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
         if (has & 1) g_logp = grads[0];
         if (has & 2) g_entropy = grads[has & 1];
         refuse("score_logprobs' backward", {&X_, &ids, &stats, &entropy, &g_logp, &g_entropy});
-        if (g_logp.defined()) g_logp = g_logp.contiguous();
-        if (g_entropy.defined()) g_entropy = g_entropy.contiguous();
+        g_logp = dense(g_logp);
+        g_entropy = dense(g_entropy);
         if (g_logp.defined() || g_entropy.defined()) {
             OnDevice on(X_);
             const Rows X = rows_of(X_);
@@ -305,8 +310,9 @@ struct ScoreLogprobs : torch::autograd::Function<ScoreLogprobs> {
     }
 };
 
-std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(const Tensor& X, const MaybeTensor& ids, double temperature,
+std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> score_logprobs(const Tensor& X, const MaybeTensor& ids_, double temperature,
                                                                               int64_t top, bool entropy, const MaybeTensor& word) {
+    const MaybeTensor ids = as_stored(ids_);
     const Tensor list = or_none(ids);
     refuse("score_logprobs", {&X, &list});
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
@@ -358,7 +364,7 @@ struct Distill : torch::autograd::Function<Distill> {
         refuse("distill_loss' backward", {&X_, &ids, &teacher, &st, &grads[0]});
         OnDevice on(X_);
         const Rows X = rows_of(X_);
-        const Tensor g = grads[0].contiguous();
+        const Tensor g = dense(grads[0]);
         Tensor dx = fresh(X.x, X.x.sizes(), X.x.scalar_type());
         if (X.n)
             check(lib.distill_bwd(X.n, X.inner, X.outer, X.stride, X.d, float_type(X.x, "X"), X.x.data_ptr(),
@@ -369,7 +375,8 @@ struct Distill : torch::autograd::Function<Distill> {
     }
 };
 
-Tensor distill_loss(const Tensor& X, const Tensor& ids, const Tensor& teacher, double temperature, const MaybeTensor& word) {
+Tensor distill_loss(const Tensor& X, const Tensor& ids_, const Tensor& teacher_, double temperature, const MaybeTensor& word) {
+    const Tensor ids = as_stored(ids_), teacher = as_stored(teacher_);
     refuse("distill_loss", {&X, &ids, &teacher});
     if (wants_graph(X)) return Distill::apply(X, ids, teacher, temperature, word);
     return distill_forward(X, ids, teacher, temperature, false, or_none(word)).first;

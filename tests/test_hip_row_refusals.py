@@ -91,3 +91,22 @@ def test_a_storage_that_was_freed_is_refused():
             x.copy_(keep)
         out = call(x)
         assert torch.equal(out, want) and torch.equal(torch.autograd.grad(out, x, up)[0], grad)
+
+
+def test_negated_views():
+    """every input, and the upstream gradients, as views that are negated on reading"""
+    x, w, ids, ts = inputs()
+    neg = lambda t: torch._neg_view(-t)                          # noqa: E731
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    x.requires_grad_(True), w.requires_grad_(True)
+    for call, args in ((layer_norm, (x, w)), (layer_norm, (x, None, w)), (lambda a: score_logprobs(a, ids).logp, (x,)),
+                       (lambda a: score_logprobs(a, ids, entropy=True).entropy, (x,)), (lambda a: distill_loss(a, ids, ts), (x,))):
+        want = call(*args)
+        up = torch.randn(want.shape, generator=torch.Generator().manual_seed(1)).to(DEV)
+        leaves = [t for t in args if t is not None]
+        grads = torch.autograd.grad(want, leaves, up, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, leaves, neg(up)), grads))
+        assert torch.equal(call(*(None if t is None else neg(t.detach()) for t in args)), want)
+    assert torch.equal(distill_loss(x, ids, neg(ts)), distill_loss(x, ids, ts))
+    assert torch.equal(score_logprobs(x, neg(ids)).logp, score_logprobs(x, ids).logp)
+    assert torch.equal(distill_loss(x, neg(ids), ts), distill_loss(x, ids, ts))

@@ -98,3 +98,16 @@ def test_tensors_without_memory_are_refused(name):
         calls(freed)[name]()
     with pytest.raises(Error, match="HIP device"):
         calls(torch.randn)[name]()
+
+
+def test_rows_of_negated_views():
+    """a view that is negated on reading (the imaginary part of a conjugate) has its values copied, whatever its strides"""
+    z = torch.complex(torch.randn(4, 6), torch.randn(4, 6))
+    for v in (z.conj().imag, z.conj().imag[..., :1], torch._neg_view(torch.randn(4, 6)), torch._neg_view(torch.randn(4, 6))[:, 1:]):
+        assert v.is_neg()
+        y, rows, inner, outer, stride = native.rows().rows_of(v)
+        assert not y.is_neg() and torch.equal(y, v) and rows == 4 and inner == 0
+        flat = torch.empty(0).set_(y.untyped_storage())
+        for r in range(4):
+            at = y.storage_offset() + r * stride
+            assert torch.equal(flat[at:at + v.shape[1]], v[r])
