@@ -5,6 +5,8 @@ tensors never leave them: there is no fallback.  A model that was never moved to
 the reference's ATen op chain instead (host_ops.py — a dispatch on where the tensors live, like the reference's own
 `models/model_utils.py:86`); a model and a batch on DIFFERENT devices raise.
 """
+import threading
+
 import torch
 
 from . import host_ops, native
@@ -18,6 +20,30 @@ def _require_cuda(t, what):
             "Move the model and the batch to the same device (model.cuda(), batch['id'].cuda(), ...).")
 
 
+class _Words:
+    """The words that IdStatus reports through, in pinned host memory that stays with the process: a kernel that is queued, or a
+    captured graph that is replayed later, may store into a word whose module is gone, and nobody else may find that store in
+    memory of theirs.  So a word (4 bytes) is handed out once; again only if its kernels are known to have finished."""
+    BLOCK = 1024
+
+    def __init__(self):
+        self._blocks, self._free, self._lock = [], [], threading.Lock()
+
+    def take(self):
+        with self._lock:
+            if not self._free:
+                self._blocks.append(torch.zeros(self.BLOCK, dtype=torch.int32).pin_memory())
+                self._free.extend(self._blocks[-1].split(1))
+            return self._free.pop()
+
+    def give_back(self, word):
+        word.zero_()
+        self._free.append(word)
+
+
+_words = _Words()
+
+
 class IdStatus:
     """The out-of-range-id report of one module, DEFERRED — the shape of the reference's GPU behaviour: nn.Embedding on a
     device (models/layers.py:20) raises nothing at the call, a device-side assert surfaces at a later synchronisation, and
@@ -29,8 +55,9 @@ class IdStatus:
         * `check_ids = "sync"` on the module polls behind every call (the rounds 1-5 behaviour: one host sync per forward).
     No allocation, fill, copy or `.item()` per call."""
 
-    def __init__(self):
+    def __init__(self, lasting=True):
         self._word = None
+        self._lasting = lasting          # False: of one call, which synchronises behind itself
 
     # a copied / pickled module (copy.deepcopy for an EMA twin, torch.save(model)) gets a FRESH report of its own: the word is
     # pinned memory tied to this process, and a plain copy of it would not be pinned
@@ -41,11 +68,11 @@ class IdStatus:
         return {}
 
     def __setstate__(self, state):
-        self._word = None
+        self.__init__()
 
     def word(self):
         if self._word is None or not self._word.is_pinned():
-            self._word = torch.zeros(1, dtype=torch.int32).pin_memory()
+            self._word = _words.take()
         return self._word
 
     def raise_if_set(self):
@@ -57,7 +84,12 @@ class IdStatus:
     def poll(self, device=None):
         if self._word is not None:
             torch.cuda.synchronize(device)
-            self.raise_if_set()
+            try:
+                self.raise_if_set()
+            finally:
+                if not self._lasting:                        # nothing that could store into it is left
+                    _words.give_back(self._word)
+                    self._word = None
 
 
 def _id_mode(check_ids, status):
@@ -66,7 +98,7 @@ def _id_mode(check_ids, status):
     if not check_ids:
         return None, False
     if status is None:                                       # a stand-alone call without a module: nothing to defer to
-        status, check_ids = IdStatus(), "sync"
+        status, check_ids = IdStatus(lasting=False), "sync"
     status.raise_if_set()
     return status, check_ids == "sync"
 
