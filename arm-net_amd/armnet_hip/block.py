@@ -56,7 +56,7 @@ class IdStatus:
     No allocation, fill, copy or `.item()` per call."""
 
     def __init__(self, lasting=True):
-        self._word = None
+        self._word, self._first = None, threading.Lock()
         self._lasting = lasting          # False: of one call, which synchronises behind itself
 
     # a copied / pickled module (copy.deepcopy for an EMA twin, torch.save(model)) gets a FRESH report of its own: the word is
@@ -72,7 +72,9 @@ class IdStatus:
 
     def word(self):
         if self._word is None or not self._word.is_pinned():
-            self._word = _words.take()
+            with self._first:                                # two first calls at once: one word
+                if self._word is None or not self._word.is_pinned():
+                    self._word = _words.take()
         return self._word
 
     def raise_if_set(self):

@@ -1,5 +1,6 @@
 """The words of the deferred id reports: memory that kernels may store into outlives whoever asked for it (no GPU: pinning is replaced)."""
 import gc
+import threading
 import weakref
 
 import pytest
@@ -70,3 +71,26 @@ def test_a_stand_alone_call_gives_its_word_back(pinned):
         assert status is mine and sync == (deferred == "sync")
         mine.poll()
         assert mine.word().data_ptr() == held                    # a module keeps its own
+
+
+def test_two_threads_have_one_report(pinned, monkeypatch):
+    """first calls of one module at once"""
+    take, meet = block._words.take, threading.Barrier(2)
+
+    def slow():
+        try:
+            meet.wait(0.2)                                       # both threads are here, if both may be
+        except threading.BrokenBarrierError:
+            pass
+        return take()
+
+    monkeypatch.setattr(block._words, "take", slow)
+    s, got = IdStatus(), []
+    ts = [threading.Thread(target=lambda: got.append(s.word())) for _ in range(2)]
+    [t.start() for t in ts], [t.join() for t in ts]
+    got[0][0] = 1
+    with pytest.raises(IndexError):
+        s.raise_if_set()
+    got[1][0] = 1
+    with pytest.raises(IndexError):
+        s.raise_if_set()
