@@ -8,6 +8,7 @@ import ctypes
 import importlib.util
 import os
 import subprocess
+import sys
 
 import torch  # noqa: F401  (must be imported first: the library binds to torch's libamdhip64.so.7)
 
@@ -54,7 +55,7 @@ class ArmnetNativeError(RuntimeError):
 def build(verbose=False):
     """Compile arm-net_amd/csrc for gfx950 with hipcc (cross-compiles without a GPU)."""
     out = None if verbose else subprocess.DEVNULL
-    subprocess.check_call(["make", "-C", CSRC, "-j8"], stdout=out)
+    subprocess.check_call(["make", "-C", CSRC, "-j8", "PYTHON=" + (sys.executable or "python3")], stdout=out)
     return LIB_PATH
 
 

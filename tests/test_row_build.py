@@ -35,6 +35,15 @@ def make(tmp_path):
     return run
 
 
+def test_the_extension_follows_torch_and_the_interpreter(make, tmp_path):
+    python = lambda says: script(tmp_path / "python", f"echo {says}")      # noqa: E731
+    assert make(python("cpython-310 2.10.0")) == (1, True)
+    assert make(python("cpython-310 2.10.0")) == (1, True)       # up to date
+    assert make(python("cpython-310 2.11.0")) == (2, True)       # another torch
+    assert make(python("cpython-312 2.11.0")) == (3, True)       # another interpreter
+    assert make(python("cpython-312 2.11.0")) == (3, True)
+
+
 def test_the_c_libraries_need_no_torch(make, tmp_path):
     assert make(script(tmp_path / "python", "exit 1")) == (0, False)
     assert make(str(tmp_path / "nowhere")) == (0, False)
