@@ -675,8 +675,14 @@ def rows():
             raise ArmnetNativeError(f"{ROWS_PATH} is missing: run `python -c 'import __graft_entry__ as g; g.build()'` "
                                     f"(or `make -C {CSRC}`). There is no CPU fallback for this path.")
         spec = importlib.util.spec_from_file_location("_armnet_rows", ROWS_PATH)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
+        rebuild = "build it again: `python -c 'import __graft_entry__ as g; g.build()'`"
+        try:
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except ImportError as e:                             # built for another interpreter or torch
+            raise ArmnetNativeError(f"{ROWS_PATH} cannot be loaded ({e}): {rebuild}") from e
+        if getattr(mod, "abi_version", None) != ABI_VERSION:
+            raise ArmnetNativeError(f"ABI version mismatch: {ROWS_PATH} {getattr(mod, 'abi_version', None)} != binding {ABI_VERSION}; {rebuild}")
         mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in EXPORTS}, ArmnetNativeError)
         _rows = mod
     return _rows

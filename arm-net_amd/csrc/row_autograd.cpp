@@ -410,6 +410,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, e.what());
         }
     });
+    m.attr("abi_version") = ARMNET_ABI_VERSION;      // of the entries' signatures, which are compiled in
     m.def("bind", &bind);
     m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
     m.def("score_logprobs", &score_logprobs, py::call_guard<py::gil_scoped_release>());

@@ -8,6 +8,8 @@ import pytest
 
 from armnet_hip import native
 
+Error = native.ArmnetNativeError
+
 
 def script(path, text):
     path.write_text("#!/bin/sh\n" + text + "\n")
@@ -52,3 +54,29 @@ def test_the_c_libraries_need_no_torch(make, tmp_path):
 def test_the_default_target_builds_both():
     text = open(os.path.join(native.CSRC, "Makefile")).read()
     assert "\nall: libs rows\n" in text and "\nlibs: $(OUT) $(IO_OUT)\n" in text
+
+
+def fresh(monkeypatch):
+    native.rows()
+    monkeypatch.setattr(native, "_rows", None)
+
+
+def test_an_extension_for_other_entries_is_refused(monkeypatch):
+    """the entries' signatures are compiled in"""
+    fresh(monkeypatch)
+    monkeypatch.setattr(native, "ABI_VERSION", native.ABI_VERSION + 1)
+    with pytest.raises(Error, match="ABI"):
+        native.rows()
+    assert native._rows is None
+
+
+def test_an_extension_that_cannot_be_loaded_says_what_to_do(monkeypatch, tmp_path):
+    fresh(monkeypatch)
+    bad = tmp_path / "_armnet_rows.so"
+    bad.write_bytes(b"not a library")
+    monkeypatch.setattr(native, "ROWS_PATH", str(bad))
+    with pytest.raises(Error, match="build"):
+        native.rows()
+    monkeypatch.setattr(native, "ROWS_PATH", str(tmp_path / "nowhere.so"))
+    with pytest.raises(Error, match="missing"):
+        native.rows()
