@@ -148,9 +148,10 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
 }
 
 // One row group: LPR lanes (NW = 1) or NW waves.  A block holds TPB / (LPR or NW * 64) of them and goes on to further rows; the next
-// row is asked for as soon as this one is unpacked, into the same registers.  Bound by memory: 65536 x 512 f32 in 51 us (5.3 TB/s),
-// 16384 x 4096 bf16 in 47 (5.7), 8000 x 8192 bf16 in 43 (6.1; a large copy moves 5.2); rows whose length is no multiple of 16 bytes
-// are slower (10007 x 2049 f16, whose last piece keeps another half of the block busy: 22 us, 3.7 TB/s).
+// row is asked for as soon as this one is unpacked, into the same registers.  Bound by memory: called again and again 65536 x 512 f32
+// takes 50 us (5.4 TB/s), 16384 x 4096 bf16 47 (5.8), 8000 x 8192 bf16 44 (5.9; a large copy moves 5.2), behind a backward 55, 49 and
+// 46; rows whose length is no multiple of 16 bytes are slower (10007 x 2049 f16, whose last piece keeps another half of the block busy:
+// 22 us, 3.7 TB/s).
 template <typename T, int LPR, int NW, int NV, int TPB>
 __global__ void __launch_bounds__(TPB) norm_fwd_kernel(NormArgs a) {
     constexpr int V = Piece<T>::N, NT = LPR < WAVE ? LPR : NW * WAVE, GROUPS = TPB / NT;
@@ -225,10 +226,10 @@ struct LaneCells {
 };
 
 // dx of a row, and the block's share of dw and db: in registers over its rows, then over its groups through LDS.  x and dy are read
-// once for all three.  Bound by memory: with the sum over the blocks 65536 x 512 f32 in 81 us (5.0 TB/s), 16384 x 4096 bf16 in 77 (5.2),
-// 8000 x 8192 bf16 in 79 (5.0); of more than 8192 values less (1500 x 16384 f32 in 70, 4.2 TB/s): one row a CU is in work, one on its
-// way.  A few hundred long rows cost what the blocks' shares cost (1000 x 10000 bf16: 26 us, of which the rows 12; 35 with the shares
-// stored value by value).
+// once for all three.  Bound by memory: behind its forward 65536 x 512 f32 takes 79 us (5.1 TB/s), 16384 x 4096 bf16 80 (5.0), 8000 x 8192
+// bf16 77 (5.1), and norm_param_kernel 5 more; of more than 8192 values less (1500 x 16384 f32 68 + 7, 4.4 TB/s): one row a CU is in
+// work, one on its way.  A few hundred long rows cost what the blocks' shares cost (1000 x 10000 bf16: 20 + 5 us where reading and writing
+// the rows takes 12; 35 in all with the shares stored value by value).
 // KEEP: what waits in LDS between the rows instead of in registers: 0 nothing, 1 the weights, 2 the sums for dw too.
 template <typename T, int LPR, int NW, int NV, int TPB, int KEEP>
 __global__ void __launch_bounds__(TPB) norm_bwd_kernel(NormArgs a) {
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(LN_SUM_WAVES * WAVE) norm_param_kernel(const f
 
 // ---- rows longer than LN_MAX_D: a block a row, read again for each step ---------------------------------------------------
 //
-// Bound by reading a row three times (of which the caches serve a part): 1000 x 20000 f32 forward in 45 us, 3.6 TB/s of what it cannot
-// do without; backward, with the parameters' gradients in a pass of their own, 105 us, 2.3 TB/s.
+// Bound by reading a row three times (of which the caches serve a part): 1000 x 20000 f32 forward in 45 us, 3.5 TB/s of what it cannot
+// do without (52 behind a backward); backward, with the parameters' gradients in a pass of their own, 61 + 29 + 7 us, 2.5 TB/s.
 
 constexpr int LN_LONG_TPB = 1024, LN_LONG_NW = LN_LONG_TPB / WAVE;
 
@@ -597,8 +598,8 @@ static NormShape norm_fwd_shape(int64_t np) {
     }
     if (np <= 128) return {WAVE, 1, 2, LN_TPB};
     if (np <= 256) return {WAVE, 4, 1, LN_TPB};
-    if (np <= 512) return {WAVE, 4, 2, LN_TPB};        // (16384 x 4096 bf16: 46 us; eight waves with one piece a lane 55)
-    if (np <= 1024) return {WAVE, 8, 2, 512};          // (8000 x 8192 bf16: 43 us; sixteen waves with one piece a lane 65)
+    if (np <= 512) return {WAVE, 4, 2, LN_TPB};        // (16384 x 4096 bf16: 47 us; eight waves with one piece a lane 55)
+    if (np <= 1024) return {WAVE, 8, 2, 512};          // (8000 x 8192 bf16: 44 us; sixteen waves with one piece a lane 65)
     if (np <= 2048) return {WAVE, 16, 2, 1024};
     return {WAVE, 16, 4, 1024};
 }

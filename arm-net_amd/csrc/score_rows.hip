@@ -174,7 +174,8 @@ __device__ __forceinline__ Sums group_sums(Sums s, float c2, float* scratch) {
 constexpr int SC_UNROLL = 2;             // pieces of 16 bytes in flight a thread (2048 x 131072 bf16: 96 us; four 106)
 constexpr int SC_BWD_UNROLL = 4;         // ... in the backward, which computes less and has no state to keep
 constexpr int SC_BUF = 512;              // candidates for the alternatives
-constexpr int SC_FEW = 128;              // so few scores are all candidates (4618 x 73 f32 with 16: 11.2 us; by their bound 13.4)
+// So few scores are all candidates (4618 x 73 with 48 alternatives: f32 11.4 us, by their bound 31.9; bf16 11.6 and 15.0)
+constexpr int SC_FEW = 128;
 
 template <int NW>
 struct TopScratch {
@@ -465,12 +466,13 @@ constexpr int score_fwd_blocks(bool top) { return top ? 6 : 8; }
 // meet at the end.  NW waves a slice; with NW = 1 a block holds four rows.  splits = 1: the answer; else the slice's sums and best
 // keys.
 //
-// Bound by reading: 2048 x 131072 bf16 in 96 us, 5.6 TB/s (a large copy moves 5.2); 65536 x 1001 f32, a wave a row, in 54 us, 4.9
-// TB/s.  A score takes nine instructions (unpack, half a max3, subtract, multiply, exp2 as four, add; the entropy two more), which
-// is 60 % of the vector unit at that rate: the maximum is taken over two pieces at once so that moving the sums to it costs a
-// sixteenth, and nothing else is done per score.  Short of that: what a row costs beside its scores (8191 x 5382 f16 20 us, 4.4
-// TB/s) and, with 50 alternatives of 256 x 1e6 bf16, 114 us for 95: the slices' searches come at the same time, at their ends, their
-// second reads are a fifth of the first, and 9 of it are score_join_kernel.
+// Bound by reading: called again and again 2048 x 131072 bf16 takes 96 us, 5.6 TB/s (a large copy moves 5.2), 65536 x 1001 f32, a wave
+// a row, 55 us, 4.8 TB/s; behind a backward 130 and 70.  A score takes nine instructions
+// (unpack, half a max3, subtract, multiply, exp2 as four, add; the entropy two more), which is 60 % of the vector unit at that rate: the
+// maximum is taken over two pieces at once so that moving the sums to it costs a sixteenth, and nothing else is done per score.  Short of
+// that: what a row costs beside its scores (8191 x 5382 f16 19 us, 4.6 TB/s; behind a backward 27) and, with 50 alternatives of
+// 256 x 1e6 bf16, 120 us for 99, and 9 for 5 in score_join_kernel: the slices' searches come at the same time, at their ends, and their
+// second reads are a fifth of the first.
 template <typename T, int NW, bool ENT, bool TOP, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB, score_fwd_blocks(TOP)) score_fwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_UNROLL;
@@ -636,8 +638,8 @@ __global__ void __launch_bounds__(SC_TPB) score_join_kernel(ScoreArgs a) {
 //
 // What a row costs beside reading it — maxima and sums across lanes, the ids, the writes — is the same instructions for one row or
 // for the 64 / LPR rows that a wave holds side by side.  A lane keeps P pieces; the piece that crosses the row's end is pulled
-// back into it, as in layer_norm.hip.  Bound by those instructions: 131072 x 64 f32 forward in 12 us (2.8 TB/s), backward in 23
-// (2.9 TB/s); 50000 x 10 f32 in 6 us each, which is little more than an empty launch.
+// back into it, as in layer_norm.hip.  Bound by those instructions: 131072 x 64 f32 forward in 12 us (2.8 TB/s), backward in 20
+// (3.4 TB/s; with the entropy 21); 50000 x 10 f32 in 3.4 and 4 us, which is little more than an empty launch.
 
 template <typename T, int LPR, int P>
 struct ShortRow {
@@ -797,7 +799,9 @@ __global__ void __launch_bounds__(SC_TPB) score_short_fwd_kernel(ScoreArgs a) {
             for (int i = 0; i < P; ++i)
 #pragma unroll
                 for (int e = 0; e < V; ++e) key[i][e] = e >= row.lo[i] ? Key::of(row.v[i][e], row.off[i] + e) : 0;
-            // few: the largest key below the last one, again and again (131072 x 64 bf16, 8 of 64: 33 us, by ranks 44)
+            // few: the largest key below the last one, again and again; by ranks any number costs the same.  131072 x 64 bf16, 8 of
+            // them 32 us and by ranks 42, but 16 of them 57 and 43, 21 71 and 43; f32 8 of 64 40 and 47, 16 of 64 68 and 47; of 30
+            // scores 5 15 and 15, 10 26 and 16: the two meet at about a sixth of the row
             if (TOP == 1 || 3 * a.top <= a.c) {
                 typename Key::type last = ~(typename Key::type)0;
                 for (int k = 0; k < a.top; ++k) {
@@ -924,8 +928,11 @@ static unsigned short_grid(int64_t rows, int lpr) {
 
 // Rows of up to 64 pieces go several to a wave: 4 lanes with one piece each, or 16 with up to four (131072 x 64 f32: 12 us, with a
 // wave a row 42; 100000 x 250 f32: 28 and 38).  Alternatives: of up to 64 scores any number; of more by repeated maxima, as long as
-// that beats a wave a row: 20000 x 100 f32 with 5 / 12 / 24 of them 10 / 15 / 24 us, a wave a row 39; 100000 x 250 with 1 / 5 / 10
-// of them bf16 33 / 50 / 73 us, f32 52 / 85 / 122, a wave a row 110 (but of 300 rows 7.8, a wave a row 5.9).
+// that beats a wave a row.  20000 x 100 f32 with 5 / 24 / 40 / 48 of them 10 / 24 / 37 / 42 us, a wave a row 40; bf16 8 / 21 / 33 / 38, a
+// wave a row 41.  Of 250 scores with 1 / 5 / 8 of them, in brackets a wave a row: 8192 rows bf16 5.9 / 8.6 / 10.7 (11.7 / 12.3 / 12.4),
+// f32 7.2 / 10.9 / 13.5 (10.8 / 11.0 / 11.1); 4096 rows bf16 5.5 / 8.0 / 9.9 (8.9 / 9.2 / 9.4), f32 6.3 / 9.5 / 11.8 (8.0 / 8.1 / 8.4); 2048
+// rows bf16 5.4 / 7.9 / 9.8 (7.5 / 7.8 / 8.0), f32 5.8 / 9.1 / 11.6 (6.7 / 6.9 / 7.0).  One rule for all types: it gives bf16 its due and
+// costs f32 up to 3 us with five to eight.
 template <typename T, bool ENT, bool TOP, bool DISTILL>
 static bool launch_short_fwd(const ScoreArgs& a, hipStream_t st) {
     constexpr int V = Piece<T>::N;
@@ -1002,7 +1009,9 @@ static int launch_score_fwd(ScoreArgs& a, void* ws, int64_t ws_bytes, hipStream_
         a.keys = (uint64_t*)(a.part + a.rows * a.splits);
     }
     // A wave a row: what a row costs beside reading it is paid once instead of by four waves.  For short rows always, for longer ones
-    // where rows alone fill the chip (8191 x 5382 f16: 27.2 us with a block a row, 23.5 with a wave; 4096 rows: 12.8, 10.3)
+    // where rows alone fill the chip.  x 5382 f16, a wave and a block a row: 8191 rows 20 and 26 us, 4096 11.8 and 14.4, 2048 8.0 and
+    // 9.2, 1000 7.0 and 6.3; f32 4096 rows 17.4 and 18.9, 2048 10.4 and 11.5; 4096 x 20001 f16 38 and 44.  The border lies above the
+    // crossing, so a wave is taken only where it wins
     const int64_t one_go = WAVE * Piece<T>::N * 4;
     if (a.c <= one_go || (a.splits == 1 && a.rows >= 4096 && a.c <= 16 * one_go))
         score_fwd_kernel<T, 1, ENT, TOP, DISTILL><<<score_grid((a.rows + 3) / 4, score_fwd_blocks(TOP)), SC_TPB, 0, st>>>(a);
@@ -1069,10 +1078,10 @@ __device__ __forceinline__ void add_listed(const int32_t* s_id, const float* s_g
 // waves a slice; NW = 1: four rows a block.  List of a group in LDS: n16 ids (padded with -1 to whole sixteens), n16 addends, the
 // table.  The first pieces and the list are on their way at the same time.
 //
-// Bound by reading and writing: 2048 x 131072 bf16 in 193 us, 5.6 TB/s; 65536 x 1001 f32 with the entropy's part in 108 us, 4.9 TB/s
-// (112 with an addend's load behind its id's).
-// 4096 x 5382 bf16 in 19 us with one id a row, 25 with 64, 26 with 100, 48 with 200, 167 with 1024 (compared with each other
-// 34, 67 and 979): what is left is the ids that come twice.
+// Bound by reading and writing: behind its forward 2048 x 131072 bf16 takes 181 us, 5.9 TB/s, 65536 x 1001 f32 with the entropy's part
+// 95 us, 5.5 TB/s (again and again 194 and 111; an addend's load behind its id's instead of beside it costs 4 %).
+// 4096 x 5382 bf16 19 us with one id a row, 24 with 64, 26 with 100, 48 with 200, 167 with 1024 (the last three with the ids compared
+// with each other 34, 67 and 979): what is left is the ids that come twice.
 template <typename T, int NW, bool ENT, bool DISTILL>
 __global__ void __launch_bounds__(SC_TPB) score_bwd_kernel(ScoreArgs a) {
     constexpr int NT = NW * WAVE, GROUPS = SC_TPB / NT, V = Piece<T>::N, U = SC_BWD_UNROLL;
@@ -1217,7 +1226,7 @@ static int launch_score_bwd(ScoreArgs& a, hipStream_t st) {
         return ARMNET_OK;
     }
     const bool narrow = a.c <= WAVE * Piece<T>::N * 4;               // a wave a row: its lanes hold it in one go
-    // slices of 16384 scores (2048 x 131072 bf16: 8192 220 us, 16384 193, 32768 211, 65536 222); few rows: down to what a block's
+    // slices of 16384 scores (2048 x 131072 bf16, again and again: 8192 220 us, 16384 194, 32768 211, 65536 222); few rows: down to what a block's
     // threads load at once
     const int64_t at_once = SC_TPB * Piece<T>::N * SC_BWD_UNROLL;
     int64_t splits = (a.c + 16383) / 16384;
