@@ -5,7 +5,8 @@ behind one.  `layer_norm` stands beside the training BatchNorm (it needs no batc
 server), `score_logprobs` and `distill_loss` beside the sparse map over a row of scores: what a row answers, and what a
 student learns from a teacher's answer.  Device tensors run the HIP kernels (float32, bfloat16, float16; fp32 arithmetic),
 host tensors the same formulas on ATen ops.  All three are differentiable once, by a backward pass; an input with a
-forward-mode tangent is refused, and so is a device call while a trace is recorded (torch.jit.trace, make_fx).
+forward-mode tangent is refused, and so are, on the device, a call while a trace is recorded (torch.jit.trace, make_fx) and a
+tensor without memory.
 """
 from typing import NamedTuple, Optional
 
